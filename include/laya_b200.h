@@ -168,6 +168,85 @@ typedef struct laya_b200_tail_args {
  * laya_b200_last_error(NULL) on the calling thread. */
 LAYA_B200_API int laya_b200_tail_noalloc(const laya_b200_tail_args* args, void* stream);
 
+/* ------------------------------------------------------------ row operators
+ * Operators of a block that a host runs on its own device buffers beside the
+ * engine (no counterpart in the reference).  They run on the current device
+ * and `stream` (a cudaStream_t, NULL: the legacy default stream), allocate
+ * nothing, do not synchronise and can be captured.  Strides are in elements
+ * between rows whose columns are contiguous; outputs must not overlap inputs
+ * other than where a buffer is said to be updated in place.  Errors: nonzero
+ * return, message from laya_b200_last_error(NULL) on the calling thread. */
+
+/* h = x + residual; y = h * rsqrt(mean(h^2) + eps) * weight; per row
+ * scale = max(max|y| * fl(1/448), 1e-12) and codes = e4m3(y / scale), the
+ * engine's activation recipe.  Sums are fp32; the norm reads the unrounded h
+ * and the codes come from the unrounded y.  Any row widths, strides and
+ * alignments (16-byte ones are faster).  A row with a NaN has NaN codes and a
+ * NaN scale. */
+typedef struct laya_b200_rms_norm_args {
+  int32_t rows;              /* 0..2^22 */
+  int32_t columns;           /* 1..16384 */
+  float eps;                 /* > 0 */
+  int32_t x_f32, residual_f32, y_f32; /* nonzero: fp32, else bf16 */
+  const void* x;
+  int64_t x_stride;
+  void* residual;            /* updated in place to h (rounded to its type), or NULL: h = x */
+  int64_t residual_stride;
+  const float* weight;       /* [columns] or NULL (1) */
+  void* y;                   /* or NULL */
+  int64_t y_stride;
+  void* codes;               /* e4m3, or NULL */
+  int64_t codes_stride;
+  float* scale;              /* [rows], with codes */
+} laya_b200_rms_norm_args;
+
+LAYA_B200_API int laya_b200_rms_norm(const laya_b200_rms_norm_args* args, void* stream);
+
+/* out[m] = x[m] W^T + bias + scaling[a] (x[m] A_a^T) B_a^T with the adapter
+ * a = index[m / rows_per_index] of row m; an index outside [0, slots) means no
+ * adapter.  bf16 operands with fp32 sums, one rounding at the end.  With
+ * `codes` the shared projection is the engine's FP8 one,
+ * (codes[m] . W8[n]) code_scale[m] weight_scale[n], while the adapters read
+ * the bf16 x.  The adapters must be finite: the rows of a tile share matrix
+ * instructions, so a NaN or infinity in one slot's B would reach the rows of
+ * other slots in its tile (x and A carry no such condition). */
+typedef struct laya_b200_lora_args {
+  int32_t rows;              /* 0..2^22 */
+  int32_t in_features;       /* a multiple of 8 (of 16 with codes) */
+  int32_t out_features;
+  int32_t slots;
+  int32_t rank;              /* a multiple of 8 up to 256; a slot of smaller rank has zeros in the rest */
+  int32_t rows_per_index;    /* rows that share one index entry: 1, or the rows of a request */
+  const void* x;             /* bf16 [rows][in_features]; rows on 16-byte boundaries */
+  int64_t x_stride;
+  const void* codes;         /* e4m3 [rows][in_features], rows on 16-byte boundaries, or NULL */
+  int64_t codes_stride;
+  const float* code_scale;   /* [rows], with codes */
+  const void* weight;        /* bf16 (e4m3 with codes) [out_features][in_features], rows on 16-byte boundaries */
+  int64_t weight_stride;
+  const float* weight_scale; /* [out_features], with codes */
+  const void* lora_a;        /* bf16 [slots][rank][in_features], contiguous, 16-byte aligned */
+  const void* lora_b;        /* bf16 [slots][out_features][rank], contiguous, 16-byte aligned */
+  const float* scaling;      /* [slots] or NULL (1) */
+  const int32_t* index;      /* [ceil(rows / rows_per_index)] */
+  const void* bias;          /* bf16 [out_features] or NULL */
+  void* out;                 /* bf16 [rows][out_features] */
+  int64_t out_stride;
+} laya_b200_lora_args;
+
+/* Bytes of workspace a call with these sizes needs on the current device. */
+LAYA_B200_API int laya_b200_lora_workspace(const laya_b200_lora_args* args, size_t* bytes);
+
+/* `workspace`: 256-byte aligned device memory for this call alone; calls (or
+ * captured graphs) that may run at the same time need one each. */
+LAYA_B200_API int laya_b200_lora_linear(const laya_b200_lora_args* args, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+/* Waits inside the operators are bounded; one that ran out makes its call's
+ * output invalid and leaves a nonzero code in the current device's status
+ * word.  This reads and clears it (synchronise the operators' streams first). */
+LAYA_B200_API int laya_b200_op_status(int32_t* status);
+
 /* Last error message of the engine (or of the last failed create when e is
  * NULL).  The pointer stays valid until the next call on the engine. */
 LAYA_B200_API const char* laya_b200_last_error(laya_b200_engine* e);

@@ -49,6 +49,15 @@ cudaError_t launch_gather_rows(float* dst, const float* src, const int* map, int
                                bool pdl);
 cudaError_t launch_tail(const TailParams& p, int batch, cudaStream_t stream, bool pdl);
 cudaError_t launch_token_gather(const TokenGatherParams& p, cudaStream_t stream, bool pdl);
+// Adapters beside a projection (lora.cu): the shrink V = s x A^T, then the
+// projection that adds V B^T; launched one behind the other on one stream.
+// bmap: 3-D map of B [slots][N][rank] bf16, box 32 x 128 x 1, 64-byte swizzle.
+cudaError_t launch_lora_shrink(const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl);
+cudaError_t launch_lora_gemm(int kind, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& bmap,
+                             const GemmParams& p, const LoraParams& lp, int bn, int split, cudaStream_t stream);
+// Status of the launches that were given no status word; reading clears it.
+cudaError_t read_op_status(uint32_t* status);
+cudaError_t launch_rms_norm(const RmsNormParams& p, cudaStream_t stream, bool pdl);
 cudaError_t launch_pack_fp8_rows(const __nv_bfloat16* w, uint8_t* q, float* scale, int rows, int k,
                                  cudaStream_t stream);
 

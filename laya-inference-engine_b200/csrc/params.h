@@ -145,6 +145,46 @@ struct QuantParams {
   int sf_cols;               // nvfp4: padded scale columns per row group
 };
 
+// Low-rank adapters beside a projection (lora.cu).  V[m] holds the adapter's
+// inner row s_a x[m] A_a^T as chunks of 32 ranks, each 128 bytes [hi 32 | lo 32].
+constexpr int kLoraMaxRank = 256;
+struct LoraParams {
+  int rows;
+  int in_features;           // multiple of 8
+  int slots;
+  int rank;                  // ranks of a slot, a multiple of 8 (unused ones are zero)
+  int chunks;                // ceil(rank / 32)
+  const int* index;          // adapter of row m at index[m / index_div]; outside [0, slots): none
+  int index_div;
+  const __nv_bfloat16* x;    // [rows][ldx]
+  long long ldx;
+  const __nv_bfloat16* a;    // [slots][rank][in_features]
+  const float* scaling;      // [slots] or null (1)
+  __nv_bfloat16* v;          // [rows][chunks][64]
+};
+
+// RMS norm rows (rms_norm.cu).  Strides in elements.
+constexpr int kRmsNormMaxColumns = 16384;
+struct RmsNormParams {
+  long long rows;
+  int d;
+  float eps;
+  const void* x;             // [rows][ldx] fp32 or bf16
+  long long ldx;
+  int x_f32;
+  void* residual;            // [rows][ldr] fp32 or bf16, updated in place, or null
+  long long ldr;
+  int residual_f32;
+  const float* w;            // [d] or null
+  void* y;                   // [rows][ldy] fp32 or bf16, or null
+  long long ldy;
+  int y_f32;
+  uint8_t* codes;            // e4m3 [rows][ldc] or null
+  long long ldc;
+  float* scale;              // [rows], with codes
+  int group;                 // threads that share a row (set by the launcher)
+};
+
 struct TailParams {
   int k;                     // options per question
   int d;

@@ -17,6 +17,7 @@ EXPORTS = ("laya_b200_create", "laya_b200_set_weight", "laya_b200_finalize", "la
            "laya_b200_capture",
            "laya_b200_release", "laya_b200_run", "laya_b200_replay_device", "laya_b200_kernel_count",
            "laya_b200_read_buffer", "laya_b200_tail_noalloc", "laya_b200_test_withhold_stage",
+           "laya_b200_rms_norm", "laya_b200_lora_workspace", "laya_b200_lora_linear", "laya_b200_op_status",
            "laya_b200_last_error", "laya_b200_destroy")
 
 
@@ -33,6 +34,27 @@ class TailArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("questions", "options", "hidden", "act_hidden")] + \
                [(n, ctypes.c_void_p) for n in ("z", "fc2_w", "fc2_b", "marker_mask", "h_sel", "a1_w", "a1_b",
                                                 "a2_w", "a2_b", "logits", "act")]
+
+
+class RmsNormArgs(ctypes.Structure):
+    """laya_b200_rms_norm_args."""
+    _fields_ = [("rows", ctypes.c_int32), ("columns", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("x_f32", ctypes.c_int32), ("residual_f32", ctypes.c_int32), ("y_f32", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("residual", ctypes.c_void_p),
+                ("residual_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("y_stride", ctypes.c_int64), ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
+                ("scale", ctypes.c_void_p)]
+
+
+class LoraArgs(ctypes.Structure):
+    """laya_b200_lora_args."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "in_features", "out_features", "slots", "rank",
+                                                "rows_per_index")] + \
+               [("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("codes", ctypes.c_void_p),
+                ("codes_stride", ctypes.c_int64), ("code_scale", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("weight_stride", ctypes.c_int64), ("weight_scale", ctypes.c_void_p), ("lora_a", ctypes.c_void_p),
+                ("lora_b", ctypes.c_void_p), ("scaling", ctypes.c_void_p), ("index", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64)]
 
 
 def make_config(cfg, max_batch, max_options):
@@ -74,6 +96,10 @@ def load():
         "laya_b200_read_buffer": (I, [P, ctypes.c_char_p, P, ctypes.c_size_t]),
         "laya_b200_tail_noalloc": (I, [ctypes.POINTER(TailArgs), P]),
         "laya_b200_test_withhold_stage": (I, [P, I]),
+        "laya_b200_rms_norm": (I, [P, P]),
+        "laya_b200_lora_workspace": (I, [P, P]),
+        "laya_b200_lora_linear": (I, [P, P, ctypes.c_size_t, P]),
+        "laya_b200_op_status": (I, [P]),
         "laya_b200_last_error": (ctypes.c_char_p, [P]),
         "laya_b200_destroy": (I, [P]),
     }
