@@ -49,12 +49,32 @@ cudaError_t launch_gather_rows(float* dst, const float* src, const int* map, int
                                bool pdl);
 cudaError_t launch_tail(const TailParams& p, int batch, cudaStream_t stream, bool pdl);
 cudaError_t launch_token_gather(const TokenGatherParams& p, cudaStream_t stream, bool pdl);
-// Adapters beside a projection (lora.cu): the shrink V = s x A^T, then the
-// projection that adds V B^T; launched one behind the other on one stream.
-// bmap: 3-D map of B [slots][N][rank] bf16, box 32 x 128 x 1, 64-byte swizzle.
-cudaError_t launch_lora_shrink(const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl);
-cudaError_t launch_lora_gemm(int kind, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& bmap,
-                             const GemmParams& p, const LoraParams& lp, int bn, int split, cudaStream_t stream);
+// Adapters beside a projection (lora.cu): the shrink V = s x A^T, which also
+// lists the adapters of every 256 rows, then the projection that adds V B^T;
+// launched one behind the other on one stream.  Tensor maps (128-byte swizzle
+// and boxes of 128 bytes of K unless said otherwise):
+struct LoraMaps {
+  CUtensorMap rows;  // X as bf16, 64 rows
+  CUtensorMap a;     // A [slots][rank][K] bf16, lora_shrink_box(rank) ranks of one slot
+  CUtensorMap w;     // weight rows: 128, or bnf / 2
+  CUtensorMap x;     // the projection's operand (X, or its codes): bn rows, or 128
+  CUtensorMap b;     // B [slots][N][rank] bf16, 32 ranks x 128 (bnf / 2) rows of one slot, 64-byte swizzle
+  CUtensorMap v;     // pairs: V as [rows][chunks * 64] bf16, 64 columns x 128 rows
+  CUtensorMap out;   // pairs with p.tma_epilogue: output, 128 bytes of columns x 32 rows
+};
+cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl);
+// Ranks of one adapter in a CTA of the shrink.
+__host__ __device__ inline int lora_shrink_box(int rank) { return rank < 64 ? (rank + 15) / 16 * 16 : 64; }
+// The projection of up to 64 rows: row tile bn, K split over clusters.
+cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
+                             int split, cudaStream_t stream);
+void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split);
+// The projection of many rows over CTA pairs: tiles of 256 rows x bnf features.
+// Without p.tma_epilogue (store epilogue only) the output may lie anywhere.
+cudaError_t launch_lora_pairs(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bnf,
+                              cudaStream_t stream);
+// Features per tile of launch_lora_pairs, or 0 where launch_lora_gemm is to be used.
+int lora_pair_plan(int kind, int M, int N, int sm_count);
 // Status of the launches that were given no status word; reading clears it.
 cudaError_t read_op_status(uint32_t* status);
 cudaError_t launch_rms_norm(const RmsNormParams& p, cudaStream_t stream, bool pdl);

@@ -28,7 +28,9 @@
 #include "params.h"
 #include "launch.h"
 #include "gemm_epilogue.cuh"
+#include "lora.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 namespace laya {
@@ -36,129 +38,352 @@ namespace laya {
 // Status of launches that were given no status word (laya_b200_op_status).
 __device__ uint32_t g_op_status;
 
+}  // namespace laya
+
+#include "lora_pair.cuh"
+
+namespace laya {
+
 namespace {
 
-// Adapter of row m, or -1 (also for every index that names no slot).
-DEVI int row_adapter(const LoraParams& p, int m) {
-  if (m >= p.rows) return -1;
-  const int a = p.index[m / p.index_div];
-  return a >= 0 && a < p.slots ? a : -1;
-}
-
 // ------------------------------------------------------------------ shrink
-// A CTA takes 16 rows, RG ranks (grid.z) and every `gridDim.y`-th of the
-// adapters that its rows use.  Its eight warps split K; a lane loads 16 bytes
-// of rows lane/4 and lane/4 + 8 and of ranks lane/4 + 8j at the same columns,
-// which are the operands of two m16n8k16 products over a permuted K (the
-// order of a sum's terms is free as long as both operands share it), so no
-// staging is needed.  The partial sums meet in shared memory in warp order.
-constexpr int kShrinkRows = 16, kShrinkWarps = 8;
+// V = s x A^T: a CTA takes 64 rows, a share of the adapters that they use, up
+// to 64 ranks and a slice of K.  The A_a of several adapters are stacked as one
+// operand, so every row meets every one of them and keeps the columns of its
+// own: no row sees another adapter's values.  The K slices of a cluster are
+// added through distributed shared memory in rank order.  The product is too
+// thin to be bound by anything but latency and the loads of its rows; it runs
+// on mma.sync with its operands staged by TMA because that takes neither tensor
+// memory nor much shared memory, so the projection's CTAs start beside it.
+constexpr int kShrinkRows = 64;
+constexpr int kShrinkRanks = 64;  // ranks of an adapter in one CTA
+constexpr int kShrinkPitch = kShrinkRanks + 4;
+constexpr int kShrinkPerSm = 3;  // CTAs of one wave on an SM: their loads in flight are what its rate comes from
 
-DEVI void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// WIDE: one adapter of more than 32 ranks at a time; else adapters that
+// together have up to 32 columns, and a stage more in the same memory.
+template <bool WIDE>
+struct ShrinkCfg {
+  static constexpr int COLS = WIDE ? 64 : 32;
+  static constexpr int STAGES = WIDE ? 3 : 4;
+  static constexpr int X_BYTES = kShrinkRows * 128, A_BYTES = COLS * 128;
+  static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
+  static constexpr int PART_BYTES = kShrinkRows * kShrinkPitch * 4;  // over the stages, between passes
+  static_assert(PART_BYTES <= PIPE_BYTES, "the partial sums fit the pipeline's memory");
+  static constexpr int SMEM = PIPE_BYTES + (2 * 128 + 264) * 4 + 128 + 1024;
+};
+
+DEVI void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                "{%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DEVI void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr)
+               : "memory");
 }
 
-template <int NT>  // rank group of 8 * NT
-__global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const LoraParams p) {
-  constexpr int RG = 8 * NT;
-  __shared__ float red[kShrinkWarps][kShrinkRows][RG];
+// The four warps that compute.
+DEVI void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Numbers the distinct non-negative values of own[] (row h * 128 + thread, 128
+// threads) in order of first appearance: ord[] of each row (-1: none), the
+// values in s_list, their count returned.  A warp's leaders look for their
+// value among the earlier warps' leaders only, so a tile of long runs costs a
+// few steps.  s_tmp, s_entry: H * 128 ints (16-byte aligned); s_cnt: H * 4.
+template <int H>
+DEVI int number_adapters(const int (&own)[H], int (&ord)[H], int* s_list, int* s_tmp, int* s_entry, int* s_cnt) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned below = (1u << lane) - 1;
+  int lead[H], entry[H], seen[H];
+  unsigned firsts[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    lead[h] = __ffs(__match_any_sync(0xffffffffu, own[h])) - 1;
+    const unsigned leaders = __ballot_sync(0xffffffffu, own[h] >= 0 && lead[h] == lane);
+    s_tmp[h * 128 + tid] = -1;
+    __syncwarp();
+    entry[h] = own[h] >= 0 && lead[h] == lane ? h * 128 + warp * 32 + __popc(leaders & below) : -1;
+    if (entry[h] >= 0) s_tmp[entry[h]] = own[h];
+  }
+  sync128();
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    seen[h] = H * 128;
+    if (entry[h] >= 0)
+      for (int j = 0; j < h * 128 + warp * 32; j += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(s_tmp + j);
+        if (v.w == own[h]) seen[h] = min(seen[h], j + 3);
+        if (v.z == own[h]) seen[h] = min(seen[h], j + 2);
+        if (v.y == own[h]) seen[h] = min(seen[h], j + 1);
+        if (v.x == own[h]) seen[h] = min(seen[h], j);
+      }
+    firsts[h] = __ballot_sync(0xffffffffu, entry[h] >= 0 && seen[h] == H * 128);
+    if (lane == 0) s_cnt[h * 4 + warp] = __popc(firsts[h]);
+  }
+  sync128();
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < 4 * H; ++w) {
+    const int h = w / 4;
+    if (w % 4 == warp && entry[h] >= 0 && seen[h] == H * 128) {
+      ord[h] = n + __popc(firsts[h] & below);
+      s_entry[entry[h]] = ord[h];
+      s_list[ord[h]] = own[h];
+    }
+    n += s_cnt[w];
+  }
+  sync128();
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    if (entry[h] >= 0 && seen[h] < H * 128) ord[h] = s_entry[seen[h]];
+    const int of_lead = __shfl_sync(0xffffffffu, ord[h], lead[h]);
+    ord[h] = own[h] >= 0 ? of_lead : -1;
+  }
+  return n;
+}
+
+// Writes the list of the 256 rows from row0 for the projection: count, adapters,
+// and each one's first and last row.  128 threads; `w`: 1536 ints of shared memory.
+DEVI void write_list(const LoraParams& p, int row0, int* w) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  int own[2], ord[2] = {-1, -1};
+  for (int h = 0; h < 2; ++h) own[h] = row_adapter(p, row0 + 128 * h + tid);
+  int *s_list = w, *s_span = w + 256;
+  const int n = number_adapters<2>(own, ord, s_list, w + 768, w + 1024, w + 1280);
+  for (int j = tid; j < n; j += 128) {
+    s_span[j] = 256;
+    s_span[256 + j] = -1;
+  }
+  sync128();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    // one lane of a warp's run speaks for it
+    const unsigned same = __match_any_sync(0xffffffffu, ord[h]);
+    if (ord[h] >= 0 && __ffs(same) - 1 == lane) {
+      atomicMin(&s_span[ord[h]], h * 128 + tid);
+      atomicMax(&s_span[256 + ord[h]], h * 128 + tid - lane + 31 - __clz(same));
+    }
+  }
+  sync128();
+  int* out = p.lists + (size_t)(row0 / 256) * kLoraListInts;
+  for (int j = tid; j < n; j += 128) {
+    out[kLoraListSlots + j] = s_list[j];
+    out[kLoraListSpans + j] = s_span[j] | s_span[256 + j] << 16;
+  }
+  if (tid == 0) out[0] = n;
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(160)
+    lora_shrink_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
+                       const LoraParams p) {
+  using C = ShrinkCfg<WIDE>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sA = smem + ST * C::X_BYTES;
+  float* part = reinterpret_cast<float*>(smem);                 // [64][kShrinkPitch], between passes
+  int* s_ord = reinterpret_cast<int*>(smem + C::PIPE_BYTES);   // [128] each row's place in the list
+  int* s_list = s_ord + 128;                                    // [128] distinct adapters
+  int* s_tmp = s_list + 128;                                    // [128] + [128] + [4]: number_adapters
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264);
+  uint64_t* empty = full + ST;
+  int* s_count = reinterpret_cast<int*>(empty + ST);
+  int* failed = s_count + 1;
   // Everything before this kernel is complete once the wait returns; the
   // projection launched behind it relies on that (its K blocks do not wait).
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row0 = blockIdx.x * kShrinkRows, r0 = blockIdx.z * RG;
-  const int mine = lane < kShrinkRows ? row_adapter(p, row0 + lane) : -1;
-  const unsigned same = __match_any_sync(0xffffffffu, mine);
-  unsigned firsts = __ballot_sync(0xffffffffu, mine >= 0 && __ffs(same) - 1 == lane);
-  const int g = lane >> 2, t8 = (lane & 3) * 8;
-  const int ra = row0 + g, rb = ra + 8;
-  const __nv_bfloat16* xa = p.x + (size_t)(ra < p.rows ? ra : 0) * p.ldx;
-  const __nv_bfloat16* xb = p.x + (size_t)(rb < p.rows ? rb : 0) * p.ldx;
-  const int steps = (p.in_features + 31) / 32;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int ordinal = 0; firsts; ++ordinal, firsts &= firsts - 1) {
-    if (ordinal % gridDim.y != blockIdx.y) continue;
-    const int slot = __shfl_sync(0xffffffffu, mine, __ffs(firsts) - 1);
-    const __nv_bfloat16* a = p.a + (size_t)slot * p.rank * p.in_features;
-    float acc[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll 2
-    for (int s = warp; s < steps; s += kShrinkWarps) {
-      const int k = s * 32 + t8;
-      const bool in = k < p.in_features;
-      const uint4 va = in && ra < p.rows ? *reinterpret_cast<const uint4*>(xa + k) : zero;
-      const uint4 vb = in && rb < p.rows ? *reinterpret_cast<const uint4*>(xb + k) : zero;
-      uint4 w[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int r = r0 + 8 * j + g;
-        w[j] = in && r < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + (size_t)r * p.in_features + k)) : zero;
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma_bf16(acc[j], va.x, vb.x, va.y, vb.y, w[j].x, w[j].y);
-        mma_bf16(acc[j], va.z, vb.z, va.w, vb.w, w[j].z, w[j].w);
-      }
-    }
-    const int c = (lane & 3) * 2;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      *reinterpret_cast<float2*>(&red[warp][g][8 * j + c]) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(&red[warp][g + 8][8 * j + c]) = make_float2(acc[j][2], acc[j][3]);
-    }
-    __syncthreads();
-    const float scaling = p.scaling ? p.scaling[slot] : 1.f;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < kShrinkRows * RG; i += 32 * kShrinkWarps) {
-      const int row = i / RG, r = r0 + i % RG;
-      // i / RG is the same for a warp's lanes or differs by whole rows; the
-      // row's adapter comes from the lane that holds it
-      const int owner = __shfl_sync(0xffffffffu, mine, row);
-      if (owner != slot || (r >> 5) >= p.chunks) continue;
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kShrinkWarps; ++w) v += red[w][row][i % RG];
-      v *= scaling;
-      const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-      // an infinite (or NaN) v has no remainder
-      const float rest = fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.f;
-      __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
-      dst[0] = hi;
-      dst[32] = __float2bfloat16_rn(rest);
-    }
-    __syncthreads();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool loader = warp == 4;
+  const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, slices = gridDim.y / groups;
+  const int group = blockIdx.y % groups, slice = blockIdx.y / groups;
+  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
+  if ((int)blockIdx.x >= tiles) {  // the CTAs behind the row tiles write the projection's lists
+    if (blockIdx.y == 0 && blockIdx.z == 0 && !loader)
+      write_list(p, ((int)blockIdx.x - tiles) * 256, reinterpret_cast<int*>(smem));
+    return;
   }
+  const int row0 = blockIdx.x * kShrinkRows, split = gridDim.z, rank = blockIdx.z;
+  const int cols = lora_shrink_box(p.rank);  // of one adapter
+  const int kblocks = (p.in_features + 63) / 64;
+  const int kb0 = rank * kblocks / split, nkb = (rank + 1) * kblocks / split - kb0;
+  const uint64_t limit = kWaitLimitNs;
+  const uint64_t pol = policy_evict_last();
+  auto load_rows = [&](int s, int k) {
+    mbar_expect_tx(&full[s], C::X_BYTES);
+    tma_load_2d(sX + s * C::X_BYTES, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
+  };
+  if (loader) {
+    if (elect_one()) {
+      for (int s = 0; s < ST; ++s) {
+        mbar_init(&full[s], 2);   // the rows, the adapters
+        mbar_init(&empty[s], 4);  // the warps that compute
+      }
+      *failed = 0;
+      fence_mbar_init();
+      for (int k = 0; k < ST && k < nkb; ++k) load_rows(k, k);
+    }
+    __syncwarp();
+  } else {
+    // ---- the tile's adapters in order of first use (the rows are on their way)
+    const int own[1] = {tid < kShrinkRows ? row_adapter(p, row0 + tid) : -1};
+    int ord[1] = {-1};
+    const int n = number_adapters<1>(own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
+    s_ord[tid] = ord[0];
+    if (tid == 0) *s_count = n;
+  }
+  __syncthreads();
+  const int n = *s_count;
+  const int u0 = (int)((long long)slice * n / slices), u1 = (int)((long long)(slice + 1) * n / slices);
+  const int per = C::COLS / cols;  // adapters of one pass
+  if (loader && u0 == u1)          // no adapter here: the rows still land before the exit
+    for (int k = 0; k < ST && k < nkb; ++k) {
+      if (elect_one()) mbar_arrive(&full[k]);
+      __syncwarp();
+      if (!warp_wait(&full[k], 0, limit) && lane == 0) atomicExch(failed, 1);
+    }
+  Ring<ST> ring;
+  uint32_t g = 0;  // K blocks before this one
+  for (int u = u0; u < u1; u += per) {
+    // (after a failure the passes still meet at their barriers)
+    const int units = u1 - u < per ? u1 - u : per, ncols = units * cols;
+    const int todo = *reinterpret_cast<volatile int*>(failed) ? 0 : nkb;
+    if (loader) {
+      for (int k = 0; k < todo; ++k, ++g, ring.next()) {
+        const int s = ring.s;
+        if (g >= ST && !warp_wait(&empty[s], ring.phase ^ 1, limit)) {
+          if (lane == 0) atomicExch(failed, 1);
+          break;
+        }
+        if (elect_one()) {
+          if (g >= ST || (int)g >= nkb) load_rows(s, k);  // (the first ones were requested above)
+          mbar_expect_tx(&full[s], ncols * 128);
+          for (int a = 0; a < units; ++a)
+            tma_load_3d(sA + s * C::A_BYTES + a * cols * 128, &amap, &full[s], (kb0 + k) * 64, group * kShrinkRanks,
+                        s_list[u + a], pol);
+        }
+        __syncwarp();
+      }
+    } else {
+      float acc[C::COLS / 8][4];
+#pragma unroll
+      for (int j = 0; j < C::COLS / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      for (int k = 0; k < todo; ++k, ring.next()) {
+        const int s = ring.s;
+        if (!warp_wait(&full[s], ring.phase, limit)) {
+          if (lane == 0) atomicExch(failed, 1);
+          break;
+        }
+        const uint32_t xs = smem_u32(sX + s * C::X_BYTES), as = smem_u32(sA + s * C::A_BYTES);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+          ldmatrix4(a, xs + sw128_offset(warp * 16 + (lane & 15), 2 * j + (lane >> 4)));
+#pragma unroll
+          for (int q = 0; q < C::COLS / 16; ++q)
+            if (16 * q < ncols) {
+              uint32_t b[4];
+              ldmatrix4(b, as + sw128_offset(16 * q + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)));
+              mma_bf16(acc[2 * q], a, b[0], b[1]);
+              mma_bf16(acc[2 * q + 1], a, b[2], b[3]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      sync128();  // every stage has been read
+      // a row keeps the columns of its own adapter
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = warp * 16 + (lane >> 2) + 8 * h, unit = s_ord[row] - u;
+        if (unit < 0 || unit >= units) continue;
+#pragma unroll
+        for (int j = 0; j < C::COLS / 8; ++j) {
+          const int c = 8 * j + (lane & 3) * 2 - unit * cols;
+          if (c >= 0 && c < cols)
+            *reinterpret_cast<float2*>(part + row * kShrinkPitch + c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+        }
+      }
+    }
+    if (split > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    if (!loader) {
+      const int t0 = rank * kShrinkRows / split, rows = (rank + 1) * kShrinkRows / split - t0;
+      const uint32_t base = smem_u32(part);
+      const int quads = cols / 4;
+      // four ranks of a row at a time; the parts of all K slices are requested
+      // before the first is added
+      for (int e = tid; e < rows * quads; e += 128) {
+        const int row = t0 + e / quads, c = e % quads * 4, r = group * kShrinkRanks + c, o = s_ord[row];
+        if (o < u || o >= u + units || (r >> 5) >= p.chunks) continue;
+        const int off = row * kShrinkPitch + c;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (split == 1) {
+          v = *reinterpret_cast<const float4*>(part + off);
+        } else {
+          float4 q[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < split) q[k] = ld_dsmem_f32x4(mapa_shared(base, k) + off * 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < split) {
+              v.x += q[k].x;
+              v.y += q[k].y;
+              v.z += q[k].z;
+              v.w += q[k].w;
+            }
+        }
+        const float f = p.scaling ? p.scaling[s_list[o]] : 1.f;
+        const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        float lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
+          lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
+        __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+      }
+    }
+    // the partial sums are read; the next pass's copies may take their place
+    fence_proxy_async_smem();
+    if (split > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  }
+  if (tid == 0 && *reinterpret_cast<volatile int*>(failed))
+    record_status(p.status ? p.status : &g_op_status, kStatusGemmFullTimeout);
 }
 
-// -------------------------------------------------------------- projection
-// B_a chunk: 128 weight rows x 32 ranks in the 64-byte swizzle TMA writes
-// (8-row groups 512 bytes apart).
-DEVI uint64_t sw64_desc(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(512 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)4 << 61;  // 64-byte swizzle
-  return d;
-}
+// ------------------------------------------------- projection for few rows
+// Up to 64 rows, bound by reading W and the adapters: the tile layout and
+// split-K of gemm.cu (weight rows on the TMEM lanes, rows of X as the MMA's N).
+// An adapter's blocks multiply only the 16-row groups between its first and
+// last row, so 64 single rows with 64 adapters cost as many narrow MMAs; four
+// builder warps prepare the V tiles, each its own blocks, loading the next
+// one's values before they wait for its stage.
+constexpr int kFewBuilders = 4;  // warps; divides STAGES (each sees every use of its stages)
 
-template <int BN, int KIND, int STAGES>
+template <int BN, int KIND>
 struct LoraCfg {
-  static constexpr int THREADS = BN >= 128 ? 256 : 128;
-  static constexpr int BUILDERS = THREADS - 64;  // threads of warps 2.. build the V tiles
+  static constexpr int STAGES = 4;
+  static constexpr int THREADS = 64 + 32 * kFewBuilders;
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
   static constexpr int PART_BYTES = BN * 128 * 4;
   static constexpr int MAIN_BYTES = PIPE_BYTES > PART_BYTES ? PIPE_BYTES : PART_BYTES;
-  static constexpr int LIST_BYTES = BN * 12;  // adapter per row, distinct adapters, activation scales
+  static constexpr int LIST_BYTES = BN * 12;  // distinct adapters, their rows, activation scales
   static constexpr int BAR_BYTES = 256;
   static constexpr int SMEM = MAIN_BYTES + BAR_BYTES + LIST_BYTES + 1024;
   static constexpr int ACCS = KIND == kKindFp8 ? 2 : 1;
@@ -187,11 +412,13 @@ DEVI void store_quad(const GemmParams& p, int m, int n, float4 v, bool vec) {
   }
 }
 
-template <int BN, int KIND, int STAGES>
-__global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 ? 2 : 1)
+template <int BN, int KIND>
+__global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                      const __grid_constant__ CUtensorMap bmap, const GemmParams p, const LoraParams lp) {
-  using C = LoraCfg<BN, KIND, STAGES>;
+  using C = LoraCfg<BN, KIND>;
+  constexpr int STAGES = C::STAGES;
+  static_assert(STAGES % kFewBuilders == 0, "builder warps and stages");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -201,30 +428,28 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
   uint64_t* vfull = empty + STAGES;
   uint64_t* vfree = vfull + STAGES;  // the producer found the stage free for an adapter block
   uint64_t* done = vfree + STAGES;
-  uint64_t* listed = done + 1;  // the tile's adapter list is complete
+  uint64_t* listed = done + 1;  // the tile's adapter list is in shared memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(listed + 1);
   uint32_t* failed = tmem_slot + 1;
-  int* s_count = reinterpret_cast<int*>(failed + 1);  // [0]: distinct adapters, [1..4]: per warp
-  static_assert((4 * STAGES + 2) * 8 + 8 + 5 * 4 <= C::BAR_BYTES, "barrier block");
-  int* s_row = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [BN] adapter of each row
-  int* s_list = s_row + BN;                                                  // [BN] distinct adapters
-  float* s_scale = reinterpret_cast<float*>(s_list + BN);                    // [BN] activation scales (fp8)
+  int* s_count = reinterpret_cast<int*>(failed + 1);
+  static_assert((4 * STAGES + 2) * 8 + 12 <= C::BAR_BYTES, "barrier block");
+  int* s_list = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [BN] distinct adapters
+  int* s_span = s_list + BN;                                                  // [BN] first | last << 16 of their rows
+  float* s_scale = reinterpret_cast<float*>(s_span + BN);                     // [BN] activation scales (fp8)
 
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int tile_n = blockIdx.x, tile_m = blockIdx.y;
+  const int tile_n = blockIdx.x;
   const int split = gridDim.z, rank = blockIdx.z;
   const int kb0 = (int)((long long)rank * p.kblocks / split);
   const int kb1 = (int)((long long)(rank + 1) * p.kblocks / split);
   const int nkb = kb1 - kb0;
   uint32_t* status = p.status ? p.status : &g_op_status;
 
-  griddep_launch_dependents();
-
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&vfull[s], C::BUILDERS);
+      mbar_init(&vfull[s], 1);
       mbar_init(&vfree[s], 1);
     }
     mbar_init(done, 1);
@@ -235,18 +460,19 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
     prefetch_tensormap(&xmap);
     prefetch_tensormap(&bmap);
   }
-  if (warp == 0) {
+  if (warp == 2) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  griddep_launch_dependents();  // only now: the next kernel may allocate tensor memory too
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem2 = tmem + (C::ACCS - 1) * BN;  // the adapters' accumulator
 
   const uint64_t limit = wait_limit(p.wait_limit_us);
-  int issued = 0;  // producer: loads issued (for the drain on failure)
+  int issued = 0;  // producer warp: loads issued (for the drain on failure)
   // This rank's share [b0, b1) of the tile's adapter blocks (adapter, chunk of
   // 32 ranks); known once `listed` has completed.
   auto blocks = [&](int& b0, int& b1) {
@@ -254,147 +480,154 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
     b0 = (int)((long long)rank * n / split);
     b1 = (int)((long long)(rank + 1) * n / split);
   };
+  // Rows [c0, c1) that block b multiplies: whole groups of 16.  The first block
+  // of the FP8 kernels takes every row, which starts their second accumulator.
+  auto span = [&](int b, int b0, int& c0, int& c1) {
+    const int sp = s_span[b / lp.chunks];
+    const bool all = KIND == kKindFp8 && b == b0;
+    c0 = all ? 0 : (sp & 0xffff) & ~15;
+    c1 = all ? BN : ((sp >> 16) + 16) & ~15;
+  };
   auto give_up = [&](uint32_t code) {
     record_status(status, code);
     atomicExch(failed, 1u);
   };
-  if (tid == 0) {
+  if (warp == 0) {
     // W, X and B_a do not wait for the shrink: whatever wrote them was
     // complete before it released this kernel.
     const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
+    Ring<STAGES> ring;
     bool ok = true;
-    for (int i = 0; i < nkb; ++i) {
-      const int s = i % STAGES;
-      if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, limit)) {
-        give_up(kStatusGemmEmptyTimeout);
-        ok = false;
-        break;
+    for (int i = 0; i < nkb; ++i, ring.next()) {
+      const int s = ring.s;
+      if (i >= STAGES && !(ok = warp_wait(&empty[s], ring.phase ^ 1, limit))) break;
+      if (elect_one()) {
+        mbar_expect_tx(&full[s], C::STAGE_BYTES);
+        tma_load_2d(sA + s * C::A_BYTES, &wmap, &full[s], (kb0 + i) * C::K_ELEMS, tile_n * 128, pol_w);
+        tma_load_2d(sB + s * C::B_BYTES, &xmap, &full[s], (kb0 + i) * C::K_ELEMS, 0, pol_x);
       }
-      mbar_expect_tx(&full[s], C::STAGE_BYTES);
-      tma_load_2d(sA + s * C::A_BYTES, &wmap, &full[s], (kb0 + i) * C::K_ELEMS, tile_n * 128, pol_w);
-      tma_load_2d(sB + s * C::B_BYTES, &xmap, &full[s], (kb0 + i) * C::K_ELEMS, tile_m * BN, pol_x);
+      __syncwarp();
       issued = i + 1;
     }
-    if (ok && !mbar_wait(listed, 0, limit)) {
-      give_up(kStatusGemmFullTimeout);
-      ok = false;
-    }
+    ok = ok && warp_wait(listed, 0, limit);
     if (ok) {
       int b0, b1;
       blocks(b0, b1);
-      for (int b = b0; b < b1; ++b) {
-        const int i = nkb + b - b0, s = i % STAGES;
-        if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, limit)) {
-          give_up(kStatusGemmEmptyTimeout);
-          break;
+      for (int b = b0; b < b1; ++b, ring.next()) {
+        const int i = nkb + b - b0, s = ring.s;
+        if (i >= STAGES && !(ok = warp_wait(&empty[s], ring.phase ^ 1, limit))) break;
+        if (elect_one()) {
+          mbar_arrive(&vfree[s]);
+          mbar_expect_tx(&full[s], 128 * 64);
+          tma_load_3d(sA + s * C::A_BYTES, &bmap, &full[s], (b % lp.chunks) * 32, tile_n * 128, s_list[b / lp.chunks],
+                      pol_w);
         }
-        mbar_arrive(&vfree[s]);
-        mbar_expect_tx(&full[s], 128 * 64);
-        tma_load_3d(sA + s * C::A_BYTES, &bmap, &full[s], (b % lp.chunks) * 32, tile_n * 128, s_list[b / lp.chunks],
-                    pol_x);
+        __syncwarp();
         issued = i + 1;
       }
     }
-  } else if (tid == 32) {
+    if (!ok && (tid & 31) == 0) give_up(kStatusGemmEmptyTimeout);
+  } else if (warp == 1) {
     const uint32_t idesc = KIND == kKindBf16 ? idesc_bf16(128, BN) : idesc_e4m3(128, BN);
-    bool ok = true;
+    const uint32_t a0 = desc_lo(smem_u32(sA)), d0 = desc_lo(smem_u32(sB));
+    Ring<STAGES> ring;
+    bool ok = true, known = false;
     int b0 = 0, b1 = 0, total = nkb;
-    for (int i = 0; i < nkb && ok; ++i) {
-      const int s = i % STAGES;
-      if (!mbar_wait(&full[s], (i / STAGES) & 1, limit)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint64_t ad = sw128_desc(smem_u32(sA + s * C::A_BYTES));
-      const uint64_t bd = sw128_desc(smem_u32(sB + s * C::B_BYTES));
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (KIND == kKindBf16)
-          umma_f16(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
-        else
-          umma_f8(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
-      }
+    for (int i = 0; i < nkb; ++i, ring.next()) {
+      const int s = ring.s;
+      if (!(ok = warp_wait(&full[s], ring.phase, limit))) break;
       // Only stages that are refilled get a release (nothing is left in
       // flight when the CTA exits); near the end that takes the block count.
-      if (i + STAGES >= nkb && total == nkb && b1 == 0) {
-        if (!mbar_wait(listed, 0, limit)) {
-          ok = false;
-          break;
-        }
+      if (i + STAGES >= nkb && !known) {
+        if (!(ok = warp_wait(listed, 0, limit))) break;
         blocks(b0, b1);
         total = nkb + b1 - b0;
-      }
-      if (i + STAGES < total) umma_commit(&empty[s]);
-    }
-    for (int b = b0; b < b1 && ok; ++b) {
-      const int i = nkb + b - b0, s = i % STAGES;
-      if (!mbar_wait(&full[s], (i / STAGES) & 1, limit) ||
-          !mbar_wait(&vfull[s], ((i - nkb) / STAGES) & 1, limit)) {
-        ok = false;
-        break;
+        known = true;
       }
       tc_fence_after();
-      const uint64_t ad = sw64_desc(smem_u32(sA + s * C::A_BYTES));
-      const uint64_t bd = sw128_desc(smem_u32(sB + s * C::B_BYTES));
-      const int left = lp.rank - (b % lp.chunks) * 32;
-      const int ksteps = left > 16 ? 2 : 1;
-      const uint32_t id2 = idesc_bf16(128, BN);
-      for (int k = 0; k < ksteps; ++k) {
-        umma_f16(tmem2, ad + 2 * k, bd + 2 * k, id2, KIND == kKindBf16 || b > b0 || k > 0);  // hi
-        umma_f16(tmem2, ad + 2 * k, bd + 4 + 2 * k, id2, 1);                                 // lo
+      if (elect_one()) {
+        const uint32_t ad = a0 + s * (C::A_BYTES >> 4), bd = d0 + s * (C::B_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (KIND == kKindBf16)
+            umma1_f16<kDesc128, kDesc128>(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
+          else
+            umma1_f8(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
+        }
+        if (i + STAGES < total) umma_commit(&empty[s]);
       }
-      if (i + STAGES < total) umma_commit(&empty[s]);
+      __syncwarp();
     }
-    if (!ok) give_up(kStatusGemmFullTimeout);
-    umma_commit(done);
+    for (int b = b0; b < b1 && ok; ++b, ring.next()) {
+      const int i = nkb + b - b0, s = ring.s;
+      if (!(ok = warp_wait(&full[s], ring.phase, limit)) ||
+          !(ok = warp_wait(&vfull[s], ((b - b0) / STAGES) & 1, limit)))
+        break;
+      tc_fence_after();
+      int c0, c1;
+      span(b, b0, c0, c1);
+      if (elect_one()) {
+        const uint32_t ad = a0 + s * (C::A_BYTES >> 4), bd = d0 + s * (C::B_BYTES >> 4);
+        const uint32_t id2 = idesc_bf16(128, c1 - c0), acc = tmem2 + c0;
+        umma1_f16<kDesc64, kDesc128>(acc, ad, bd, id2, KIND == kKindBf16 || b > b0);  // hi
+        umma1_f16<kDesc64, kDesc128>(acc, ad, bd + 4, id2, 1);                        // lo
+        if (lp.rank - (b % lp.chunks) * 32 > 16) {
+          umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 2, id2, 1);
+          umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 6, id2, 1);
+        }
+        if (i + STAGES < total) umma_commit(&empty[s]);
+      }
+      __syncwarp();
+    }
+    if (!ok && (tid & 31) == 0) give_up(kStatusGemmFullTimeout);
+    if (elect_one()) umma_commit(done);
+    __syncwarp();
   } else if (warp >= 2) {
-    // ---- the tile's adapters in order of first use, then their V tiles
-    static_assert(BN <= C::BUILDERS, "a builder thread per row");
+    // ---- the list, then the V tiles: rows of other adapters are zero
+    constexpr int BUILDERS = 32 * kFewBuilders;
     const int bt = tid - 64, lane = tid & 31, bw = bt >> 5;
-    int owner = -1;
-    if (bt < BN) {
-      owner = row_adapter(lp, tile_m * BN + bt);
-      s_row[bt] = owner;
+    const int own0 = row_adapter(lp, lane), own1 = BN > 32 ? row_adapter(lp, lane + 32) : -1;
+    griddep_wait();  // the list and V
+    const int n = min(lp.lists[0], BN);
+    if (bt < n) {
+      s_list[bt] = lp.lists[kLoraListSlots + bt];
+      s_span[bt] = lp.lists[kLoraListSpans + bt];
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(C::BUILDERS) : "memory");
-    bool first = bt < BN && owner >= 0;
-    for (int j = 0; first && j < bt; ++j) first = s_row[j] != owner;
-    const unsigned bal = __ballot_sync(0xffffffffu, first);
-    if (lane == 0 && bw < 4) s_count[1 + bw] = __popc(bal);
-    asm volatile("bar.sync 1, %0;" ::"n"(C::BUILDERS) : "memory");
-    constexpr int ROW_WARPS = (BN + 31) / 32;
-    int before = 0, n = 0;
-    for (int j = 0; j < ROW_WARPS; ++j) {
-      if (j < bw) before += s_count[1 + j];
-      n += s_count[1 + j];
-    }
-    if (first) s_list[before + __popc(bal & ((1u << lane) - 1))] = owner;
     if (bt == 0) s_count[0] = n;
-    asm volatile("bar.sync 1, %0;" ::"n"(C::BUILDERS) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(BUILDERS) : "memory");
     if (bt == 0) mbar_arrive(listed);
     int b0, b1;
     blocks(b0, b1);
-    griddep_wait();  // V
-    for (int b = b0; b < b1; ++b) {
-      const int i = nkb + b - b0, s = i % STAGES;
+    const int j = lane & 7;  // 16-byte chunk of a V row
+    for (int b = b0 + bw; b < b1; b += kFewBuilders) {
+      const int s = (nkb + b - b0) % STAGES, c = b % lp.chunks, slot = s_list[b / lp.chunks];
+      const int ksteps = lp.rank - c * 32 > 16 ? 2 : 1;
+      int c0, c1;
+      span(b, b0, c0, c1);
+      uint4 v[BN / 4];
+#pragma unroll
+      for (int u = 0; u < BN / 4; ++u) {
+        const int row = c0 + u * 4 + (lane >> 3);
+        const int o0 = __shfl_sync(0xffffffffu, own0, row & 31), o1 = __shfl_sync(0xffffffffu, own1, row & 31);
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (row < c1 && (row < 32 ? o0 : o1) == slot && (j & 3) < 2 * ksteps)
+          v[u] = *reinterpret_cast<const uint4*>(lp.v + ((size_t)row * lp.chunks + c) * 64 + j * 8);
+      }
       // (the builders cannot wait on `empty` themselves: they have not followed
       // its phases through the K blocks, and a parity names every second one)
-      if (!mbar_wait(&vfree[s], ((i - nkb) / STAGES) & 1, limit)) {
-        give_up(kStatusGemmEmptyTimeout);
+      if (!warp_wait(&vfree[s], ((b - b0) / STAGES) & 1, limit)) {
+        if (lane == 0) give_up(kStatusGemmEmptyTimeout);
         break;
       }
-      const int slot = s_list[b / lp.chunks], c = b % lp.chunks;
       uint8_t* dst = sB + s * C::B_BYTES;
-      for (int u = bt; u < BN * 8; u += C::BUILDERS) {
-        const int row = u >> 3, j = u & 7;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (s_row[row] == slot)
-          v = *reinterpret_cast<const uint4*>(lp.v + ((size_t)(tile_m * BN + row) * lp.chunks + c) * 64 + j * 8);
-        *reinterpret_cast<uint4*>(dst + sw128_offset(row, j)) = v;
+#pragma unroll
+      for (int u = 0; u < BN / 4; ++u) {
+        const int row = u * 4 + (lane >> 3);
+        if (c0 + row < c1) *reinterpret_cast<uint4*>(dst + sw128_offset(row, j)) = v[u];
       }
       fence_proxy_async_smem();
-      mbar_arrive(&vfull[s]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[s]);
     }
   }
   __syncwarp();
@@ -402,27 +635,25 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
   // ---- epilogue: TMEM -> fp32 tile [BN][128] -> cluster reduction -> store
   griddep_wait();
   if (KIND == kKindFp8)
-    for (int i = tid; i < BN; i += C::THREADS) s_scale[i] = tile_m * BN + i < p.M ? p.a_scale[tile_m * BN + i] : 0.f;
-  if (!mbar_wait(done, 0, limit)) give_up(kStatusGemmDoneTimeout);
+    for (int i = tid; i < BN; i += C::THREADS) s_scale[i] = i < p.M ? p.a_scale[i] : 0.f;
+  if (!warp_wait(done, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
   tc_fence_after();
   __syncthreads();
   const bool gpath = split > 1 && p.partials != nullptr;
   float* part = reinterpret_cast<float*>(smem);
-  if (gpath) part = p.partials + ((size_t)(tile_m * gridDim.x + tile_n) * split + rank) * BN * 128;
+  if (gpath) part = p.partials + ((size_t)tile_n * split + rank) * BN * 128;
   {
     int b0, b1;
     blocks(b0, b1);
     const bool second = KIND == kKindFp8 && b1 > b0;
     const int lq = warp & 3;
-    constexpr int HALVES = C::THREADS / 128;
-    constexpr int COLS = BN / HALVES;
-    const int c0 = (warp >> 2) * COLS;
     const int lr = lq * 32 + (tid & 31);  // weight row of the tile
     const uint32_t lane_addr = (uint32_t)(lq * 32) << 16;
     const float ws = KIND == kKindFp8 && tile_n * 128 + lr < p.N ? p.w_scale[tile_n * 128 + lr] : 1.f;
-    constexpr int W = COLS < 32 ? 16 : 32;
+    constexpr int W = BN < 32 ? 16 : 32;
+    if (warp < 4)
 #pragma unroll 1
-    for (int c = c0; c < c0 + COLS; c += W) {
+    for (int c = 0; c < BN; c += W) {
       uint32_t r[W], q[W];
       if constexpr (W == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
       if (second) {
@@ -456,7 +687,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
     for (int item = tid; item < (t1 - t0) * 16; item += C::THREADS) {
       const int tl = t0 + (item >> 4);
       const int q4 = rope ? ((item >> 3) & 1) * 64 + (item & 7) * 4 : (item & 15) * 4;
-      const int m = tile_m * BN + tl, n = tile_n * 128 + q4;
+      const int m = tl, n = tile_n * 128 + q4;
       if (m >= p.M) continue;
       const int off = tl * 128 + q4;
       EpiPre pre;
@@ -472,7 +703,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
         for (int u = 0; u < 8; ++u)
           if (u < split) {
             if (gpath) {
-              const float* src = p.partials + ((size_t)(tile_m * gridDim.x + tile_n) * split + u) * BN * 128 + off;
+              const float* src = p.partials + ((size_t)tile_n * split + u) * BN * 128 + off;
               va[u] = __ldcg(reinterpret_cast<const float4*>(src));
               vb[u] = __ldcg(reinterpret_cast<const float4*>(src + pair));
             } else {
@@ -507,16 +738,16 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND, STAGES>::THREADS, BN == 128 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) tmem_dealloc(tmem, C::TMEM_COLS);
+  if (warp == 2) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
 // ------------------------------------------------------------------ host side
 
-template <int BN, int KIND, int STAGES>
-cudaError_t launch_one(const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& bmap, const GemmParams& p,
-                       const LoraParams& lp, int split, cudaStream_t stream) {
-  using C = LoraCfg<BN, KIND, STAGES>;
-  auto kern = lora_gemm_kernel<BN, KIND, STAGES>;
+template <int BN, int KIND>
+cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int split,
+                       cudaStream_t stream) {
+  using C = LoraCfg<BN, KIND>;
+  auto kern = lora_gemm_kernel<BN, KIND>;
   // Function attributes are per device: set them once for each device used.
   static std::mutex mu;
   static uint64_t ready = 0;
@@ -532,7 +763,7 @@ cudaError_t launch_one(const CUtensorMap& wmap, const CUtensorMap& xmap, const C
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N + 127) / 128, (p.M + BN - 1) / BN, split);
+  cfg.gridDim = dim3((p.N + 127) / 128, 1, split);
   cfg.blockDim = dim3(C::THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
@@ -548,61 +779,98 @@ cudaError_t launch_one(const CUtensorMap& wmap, const CUtensorMap& xmap, const C
     cfg.numAttrs = 2;
   }
   cfg.attrs = attrs;
-  return cudaLaunchKernelEx(&cfg, kern, wmap, xmap, bmap, p, lp);
+  return cudaLaunchKernelEx(&cfg, kern, maps.w, maps.x, maps.b, p, lp);
 }
 
 template <int KIND>
-cudaError_t dispatch_bn(int bn, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& bmap,
-                        const GemmParams& p, const LoraParams& lp, int split, cudaStream_t st) {
+cudaError_t dispatch_bn(int bn, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int split,
+                        cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_one<16, KIND, 4>(wmap, xmap, bmap, p, lp, split, st);
-    case 32: return launch_one<32, KIND, 4>(wmap, xmap, bmap, p, lp, split, st);
-    case 64: return launch_one<64, KIND, 4>(wmap, xmap, bmap, p, lp, split, st);
-    case 128: return launch_one<128, KIND, 3>(wmap, xmap, bmap, p, lp, split, st);
+    case 16: return launch_one<16, KIND>(maps, p, lp, split, st);
+    case 32: return launch_one<32, KIND>(maps, p, lp, split, st);
+    case 64: return launch_one<64, KIND>(maps, p, lp, split, st);
   }
   return cudaErrorInvalidValue;
 }
 
-template <int NT>
-cudaError_t shrink_one(const LoraParams& p, int slices, cudaStream_t stream, bool pdl) {
+}  // namespace
+
+namespace {
+
+template <bool WIDE>
+cudaError_t shrink_one(const LoraMaps& maps, const LoraParams& p, dim3 grid, cudaStream_t stream, bool pdl) {
+  constexpr int kSmem = ShrinkCfg<WIDE>::SMEM;
+  auto kern = lora_shrink_kernel<WIDE>;
+  static std::mutex mu;
+  static uint64_t ready = 0;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!(ready >> dev & 1)) {
+      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      if (err != cudaSuccess) return err;
+      ready |= uint64_t(1) << dev;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.rows + kShrinkRows - 1) / kShrinkRows, slices, (p.rank + 8 * NT - 1) / (8 * NT));
-  cfg.blockDim = dim3(32 * kShrinkWarps, 1, 1);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(160, 1, 1);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, lora_shrink_kernel<NT>, p);
+  cudaLaunchAttribute attrs[2];
+  cfg.attrs = attrs;
+  if (pdl) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (grid.z > 1) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = 1;
+    attrs[cfg.numAttrs].val.clusterDim.y = 1;
+    attrs[cfg.numAttrs++].val.clusterDim.z = grid.z;
+  }
+  return cudaLaunchKernelEx(&cfg, kern, maps.rows, maps.a, p);
 }
 
 }  // namespace
 
-cudaError_t launch_lora_shrink(const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl) {
+cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl) {
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
-      p.index_div < 1)
+      p.index_div < 1 || !p.lists)
     return cudaErrorInvalidValue;
-  // Few rows: the adapters of a row tile are spread over CTAs (16 single rows
-  // may each bring one), up to about two CTAs per SM.
-  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
-  int slices = 2 * sm_count / tiles;
-  if (slices > kShrinkRows) slices = kShrinkRows;
-  if (slices > p.rows) slices = p.rows;
-  if (slices > p.slots) slices = p.slots;
-  if (slices < 1) slices = 1;
-  if (p.rank <= 16) return shrink_one<2>(p, slices, stream, pdl);
-  if (p.rank <= 32) return shrink_one<4>(p, slices, stream, pdl);
-  return shrink_one<8>(p, slices, stream, pdl);
+  // One wave of CTAs: few rows (single rows of many requests) may each bring
+  // an adapter, so their adapters are spread first; many rows share a few, and
+  // there only K is split.
+  const bool wide = p.rank > 32;
+  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows, groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks;
+  const int kblocks = (p.in_features + 63) / 64, per = (wide ? 64 : 32) / lora_shrink_box(p.rank);
+  const int room = std::max(1, kShrinkPerSm * sm_count / (tiles * groups));
+  const int most = std::min(p.slots, std::min(p.rows, kShrinkRows));
+  const int slices = p.rows <= 256 ? std::min(room, (most + per - 1) / per) : 1;
+  int split = 1;
+  while (split < 8 && 2 * split <= kblocks && 2 * split * slices <= room) split *= 2;
+  const dim3 grid(tiles + (p.rows + 255) / 256, groups * slices, split);
+  return wide ? shrink_one<true>(maps, p, grid, stream, pdl) : shrink_one<false>(maps, p, grid, stream, pdl);
 }
 
-cudaError_t launch_lora_gemm(int kind, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& bmap,
-                             const GemmParams& p, const LoraParams& lp, int bn, int split, cudaStream_t stream) {
-  if (p.M < 1 || p.N < 1 || split < 1 || split > 8 || split > p.kblocks || lp.rows != p.M)
+cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
+                             int split, cudaStream_t stream) {
+  if (p.M < 1 || p.M > bn || p.N < 1 || split < 1 || split > 8 || split > p.kblocks || lp.rows != p.M)
     return cudaErrorInvalidValue;
-  if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, wmap, xmap, bmap, p, lp, split, stream);
-  if (kind == kKindFp8) return dispatch_bn<kKindFp8>(bn, wmap, xmap, bmap, p, lp, split, stream);
+  if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, maps, p, lp, split, stream);
+  if (kind == kKindFp8) return dispatch_bn<kKindFp8>(bn, maps, p, lp, split, stream);
   return cudaErrorInvalidValue;
+}
+
+// Row tile and K split of launch_lora_gemm.  Clusters of a power of two up to
+// about two CTAs per SM (a cluster of seven packs badly on the GPCs).
+void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split) {
+  *bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  const int tiles = (N + 127) / 128;
+  *split = 1;
+  while (*split < 8 && 2 * *split <= kblocks && 2 * *split * tiles <= 2 * sm_count) *split *= 2;
 }
 
 cudaError_t read_op_status(uint32_t* status) {

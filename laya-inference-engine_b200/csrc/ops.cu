@@ -52,20 +52,12 @@ int sm_count_of_current() {
   return n;
 }
 
-bool rows_map(CUtensorMap* m, const void* ptr, int rows, int cols, long long ld, int esize, int box_rows) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * esize};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / esize), (cuuint32_t)box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return get_encode_fn()(m, esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
-                         const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 struct LoraPlan {
-  int kind, kblocks, bn, split;
-  size_t v_bytes, partial_bytes;
+  int kind, kblocks;
+  int bnf;        // features per tile of the pair kernel, or 0:
+  int bn, split;  // row tile and K split of the kernel for few rows
+  size_t v_bytes, list_bytes, partial_bytes;
+  size_t bytes() const { return v_bytes + list_bytes + partial_bytes; }
 };
 
 constexpr int kMaxRows = 1 << 22, kMaxFeatures = 1 << 20;
@@ -87,13 +79,17 @@ bool lora_plan(const laya_b200_lora_args* a, int sm_count, LoraPlan* plan) {
   plan->kind = a->codes ? kKindFp8 : kKindBf16;
   const int ke = gemm_k_elems(plan->kind);
   plan->kblocks = (a->in_features + ke - 1) / ke;
-  const int n128 = (a->out_features + 127) / 128 * 128;
-  gemm_plan(a->rows > 0 ? a->rows : 1, n128, plan->kblocks, sm_count, &plan->bn, &plan->split);
-  plan->v_bytes = ((size_t)a->rows * ((a->rank + 31) / 32) * 128 + 255) / 256 * 256;
-  plan->partial_bytes =
-      plan->split > 1
-          ? (size_t)(n128 / 128) * ((a->rows + plan->bn - 1) / plan->bn) * plan->split * plan->bn * 128 * sizeof(float)
-          : 0;
+  const int rows = a->rows > 0 ? a->rows : 1;
+  auto align_up = [](size_t x) { return (x + 255) / 256 * 256; };
+  plan->v_bytes = align_up((size_t)rows * ((a->rank + 31) / 32) * 128);
+  plan->list_bytes = align_up((size_t)((rows + 255) / 256) * kLoraListInts * sizeof(int));
+  plan->partial_bytes = 0;
+  plan->bnf = lora_pair_plan(plan->kind, rows, a->out_features, sm_count);
+  if (!plan->bnf) {
+    lora_few_plan(rows, a->out_features, plan->kblocks, sm_count, &plan->bn, &plan->split);
+    if (plan->split > 1)
+      plan->partial_bytes = (size_t)((a->out_features + 127) / 128) * plan->split * plan->bn * 128 * sizeof(float);
+  }
   return true;
 }
 
@@ -147,7 +143,7 @@ extern "C" int laya_b200_lora_workspace(const laya_b200_lora_args* a, size_t* by
     const int sms = sm_count_of_current();
     LoraPlan plan;
     if (!sms || !lora_plan(a, sms, &plan)) return 1;
-    *bytes = plan.v_bytes + plan.partial_bytes;
+    *bytes = plan.bytes();
     return 0;
   } catch (...) {
     return 1;
@@ -181,23 +177,32 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     const int sms = sm_count_of_current();
     if (!sms || !lora_plan(a, sms, &plan)) return 1;
     if (!workspace || !aligned(workspace, 256)) return reject("workspace must be a 256-byte aligned device pointer");
-    if (workspace_bytes < plan.v_bytes + plan.partial_bytes) return reject("workspace is too small");
+    if (workspace_bytes < plan.bytes()) return reject("workspace is too small");
     if (!get_encode_fn()) return reject("cuTensorMapEncodeTiled is unavailable");
 
     const int M = a->rows, N = a->out_features, K = a->in_features;
-    CUtensorMap wmap, xmap, bmap;
+    const int chunks = (a->rank + 31) / 32;
+    LoraMaps maps{};
     const void* operand = a->codes ? a->codes : a->x;
     const long long ldo = a->codes ? a->codes_stride : a->x_stride;
-    bool ok = rows_map(&wmap, a->weight, N, K, a->weight_stride, wsize, 128) &&
-              rows_map(&xmap, operand, M, K, ldo, wsize, plan.bn) &&
-              lora_b_map(&bmap, a->lora_b, a->slots, N, a->rank);
+    const int wbox = plan.bnf ? plan.bnf / 2 : 128;
+    // rows of the output that take TMA stores
+    const bool tma_out = plan.bnf && aligned(a->out, 16) && a->out_stride % 8 == 0;
+    bool ok = rows_map(&maps.rows, a->x, M, K, a->x_stride, 2, 64) &&
+              slots_map(&maps.a, a->lora_a, a->slots, a->rank, K, 64, lora_shrink_box(a->rank),
+                        CU_TENSOR_MAP_SWIZZLE_128B) &&
+              rows_map(&maps.w, a->weight, N, K, a->weight_stride, wsize, wbox) &&
+              rows_map(&maps.x, operand, M, K, ldo, wsize, plan.bnf ? 128 : plan.bn) &&
+              slots_map(&maps.b, a->lora_b, a->slots, N, a->rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B) &&
+              (!plan.bnf || rows_map(&maps.v, workspace, M, chunks * 64, chunks * 64, 2, 128)) &&
+              (!tma_out || rows_map(&maps.out, a->out, M, N, a->out_stride, 2, 32));
     if (!ok) return reject("a tensor map was rejected");
     LoraParams lp{};
     lp.rows = M;
     lp.in_features = K;
     lp.slots = a->slots;
     lp.rank = a->rank;
-    lp.chunks = (a->rank + 31) / 32;
+    lp.chunks = chunks;
     lp.index = a->index;
     lp.index_div = a->rows_per_index;
     lp.x = static_cast<const __nv_bfloat16*>(a->x);
@@ -211,16 +216,19 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     p.K = K;
     p.kblocks = plan.kblocks;
     p.epilogue = kEpiStore;
+    p.tma_epilogue = tma_out;
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.ldo = (int)a->out_stride;
     p.bias = static_cast<const __nv_bfloat16*>(a->bias);
     p.a_scale = a->code_scale;
     p.w_scale = a->weight_scale;
-    if (plan.split > 1) p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
+    lp.lists = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
+    if (plan.partial_bytes) p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t err = launch_lora_shrink(lp, sms, st, true);
+    cudaError_t err = launch_lora_shrink(maps, lp, sms, st, true);
     if (err != cudaSuccess) return reject("adapter shrink launch", err);
-    err = launch_lora_gemm(plan.kind, wmap, xmap, bmap, p, lp, plan.bn, plan.split, st);
+    err = plan.bnf ? launch_lora_pairs(plan.kind, maps, p, lp, plan.bnf, st)
+                   : launch_lora_gemm(plan.kind, maps, p, lp, plan.bn, plan.split, st);
     return err == cudaSuccess ? 0 : reject("adapter projection launch", err);
   } catch (...) {
     return 1;

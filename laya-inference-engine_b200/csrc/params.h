@@ -148,6 +148,8 @@ struct QuantParams {
 // Low-rank adapters beside a projection (lora.cu).  V[m] holds the adapter's
 // inner row s_a x[m] A_a^T as chunks of 32 ranks, each 128 bytes [hi 32 | lo 32].
 constexpr int kLoraMaxRank = 256;
+// Adapters that 256 rows use: their count, [256] adapters, [256] first row | last row << 16.
+constexpr int kLoraListSlots = 4, kLoraListSpans = 260, kLoraListInts = 516;
 struct LoraParams {
   int rows;
   int in_features;           // multiple of 8
@@ -161,6 +163,8 @@ struct LoraParams {
   const __nv_bfloat16* a;    // [slots][rank][in_features]
   const float* scaling;      // [slots] or null (1)
   __nv_bfloat16* v;          // [rows][chunks][64]
+  int* lists;                // [ceil(rows / 256)][kLoraListInts]
+  uint32_t* status;          // device-visible status word, or null
 };
 
 // RMS norm rows (rms_norm.cu).  Strides in elements.
