@@ -54,7 +54,7 @@ cudaError_t launch_token_gather(const TokenGatherParams& p, cudaStream_t stream,
 // launched one behind the other on one stream.  Tensor maps (128-byte swizzle
 // and boxes of 128 bytes of K unless said otherwise):
 struct LoraMaps {
-  CUtensorMap rows;  // X as bf16, 64 rows
+  CUtensorMap rows;  // X as bf16, lora_shrink_rows(rows) rows
   CUtensorMap a;     // A [slots][rank][K] bf16, lora_shrink_box(rank) ranks of one slot
   CUtensorMap w;     // weight rows: 128, or bnf / 2
   CUtensorMap x;     // the projection's operand (X, or its codes): bn rows, or 128
@@ -63,7 +63,8 @@ struct LoraMaps {
   CUtensorMap out;   // pairs with p.tma_epilogue: output, 128 bytes of columns x 32 rows
 };
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl);
-// Ranks of one adapter in a CTA of the shrink.
+// Rows, and ranks of one adapter, in a CTA of the shrink.
+inline int lora_shrink_rows(int rows) { return rows <= 64 ? 64 : 128; }
 __host__ __device__ inline int lora_shrink_box(int rank) { return rank < 64 ? (rank + 15) / 16 * 16 : 64; }
 // The projection of up to 64 rows: row tile bn, K split over clusters.
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,

@@ -47,44 +47,25 @@ namespace laya {
 namespace {
 
 // ------------------------------------------------------------------ shrink
-// V = s x A^T: a CTA takes 64 rows, a share of the adapters that they use, up
-// to 64 ranks and a slice of K.  The A_a of several adapters are stacked as one
-// operand, so every row meets every one of them and keeps the columns of its
-// own: no row sees another adapter's values.  The K slices of a cluster are
-// added through distributed shared memory in rank order.  The product is too
-// thin to be bound by anything but latency and the loads of its rows; it runs
-// on mma.sync with its operands staged by TMA because that takes neither tensor
-// memory nor much shared memory, so the projection's CTAs start beside it.
-constexpr int kShrinkRows = 64;
-constexpr int kShrinkRanks = 64;  // ranks of an adapter in one CTA
+// V = s x A^T on tcgen05: a CTA takes 128 rows (the TMEM lanes), a share of the
+// adapters that they use, up to 64 ranks and a slice of K.  The A_a of up to
+// kShrinkCols / ranks adapters are stacked as one B operand, so the rows are
+// read once for all of them; every row meets every adapter of the pass and
+// keeps the columns of its own, so that no row sees another adapter's values.
+// The K slices of a cluster are added through distributed shared memory in
+// rank order.  Bound by the loads (rows and adapters once each) and, for few
+// rows, by the latency of two dependent loads and the exchange.  (On mma.sync,
+// small enough to share its SM with the projection, it took 15 us for 8,192
+// rows and 41 K blocks: too few bytes in flight.)
+constexpr int kShrinkRows = 128;
+constexpr int kShrinkRanks = 64;   // ranks of an adapter in one CTA
+constexpr int kShrinkCols = 256;   // columns of one pass
+constexpr int kShrinkStages = 4;
 constexpr int kShrinkPitch = kShrinkRanks + 4;
-constexpr int kShrinkPerSm = 3;  // CTAs of one wave on an SM: their loads in flight are what its rate comes from
-
-// WIDE: one adapter of more than 32 ranks at a time; else adapters that
-// together have up to 32 columns, and a stage more in the same memory.
-template <bool WIDE>
-struct ShrinkCfg {
-  static constexpr int COLS = WIDE ? 64 : 32;
-  static constexpr int STAGES = WIDE ? 3 : 4;
-  static constexpr int X_BYTES = kShrinkRows * 128, A_BYTES = COLS * 128;
-  static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
-  static constexpr int PART_BYTES = kShrinkRows * kShrinkPitch * 4;  // over the stages, between passes
-  static_assert(PART_BYTES <= PIPE_BYTES, "the partial sums fit the pipeline's memory");
-  static constexpr int SMEM = PIPE_BYTES + (2 * 128 + 264) * 4 + 128 + 1024;
-};
-
-DEVI void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-DEVI void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(saddr)
-               : "memory");
-}
+constexpr int kShrinkXBytes = kShrinkRows * 128, kShrinkABytes = kShrinkCols * 128;
+constexpr int kShrinkPipe = kShrinkStages * (kShrinkXBytes + kShrinkABytes);
+static_assert(kShrinkRows * kShrinkPitch * 4 <= kShrinkPipe, "the partial sums lie over the stages");
+constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264) * 4 + 128 + 1024;
 
 // The four warps that compute.
 DEVI void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -177,11 +158,245 @@ DEVI void write_list(const LoraParams& p, int row0, int* w) {
   if (tid == 0) out[0] = n;
 }
 
-template <bool WIDE>
-__global__ void __launch_bounds__(160)
+__global__ void __launch_bounds__(192)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
                        const LoraParams p) {
-  using C = ShrinkCfg<WIDE>;
+  constexpr int ST = kShrinkStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sA = smem + ST * kShrinkXBytes;
+  float* part = reinterpret_cast<float*>(smem);               // [128][kShrinkPitch], between passes
+  int* s_ord = reinterpret_cast<int*>(smem + kShrinkPipe);   // [128] each row's place in the list
+  int* s_list = s_ord + 128;                                  // [128] distinct adapters
+  int* s_tmp = s_list + 128;                                  // [128] + [128] + [4]: number_adapters
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264);
+  uint64_t* empty = full + ST;
+  uint64_t* done = empty + ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* s_count = reinterpret_cast<int*>(tmem_slot + 1);
+  int* failed = s_count + 1;
+  // Everything before this kernel is complete once the wait returns; the
+  // projection launched behind it relies on that (its K blocks do not wait).
+  griddep_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
+  if ((int)blockIdx.x >= tiles) {  // the CTAs behind the row tiles write the projection's lists
+    griddep_launch_dependents();
+    if (blockIdx.y == 0 && blockIdx.z == 0 && warp < 4)
+      write_list(p, ((int)blockIdx.x - tiles) * 256, reinterpret_cast<int*>(smem));
+    return;
+  }
+  const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, slices = gridDim.y / groups;
+  const int group = blockIdx.y % groups, slice = blockIdx.y / groups;
+  const int row0 = blockIdx.x * kShrinkRows, split = gridDim.z, rank = blockIdx.z;
+  const int cols = lora_shrink_box(p.rank);  // of one adapter
+  const int kblocks = (p.in_features + 63) / 64;
+  const int kb0 = rank * kblocks / split, nkb = (rank + 1) * kblocks / split - kb0;
+  const uint64_t limit = kWaitLimitNs;
+  const uint64_t pol = policy_evict_last();
+  auto load_rows = [&](int s, int k) {
+    mbar_expect_tx(&full[s], kShrinkXBytes);
+    tma_load_2d(sX + s * kShrinkXBytes, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
+  };
+  if (warp == 4) {
+    if (elect_one()) {
+      for (int s = 0; s < ST; ++s) {
+        mbar_init(&full[s], 2);  // the rows, the adapters
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(done, 1);
+      *failed = 0;
+      fence_mbar_init();
+      for (int k = 0; k < ST && k < nkb; ++k) load_rows(k, k);
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    tmem_alloc(tmem_slot, kShrinkCols);
+    tmem_relinquish();
+  } else {
+    // ---- the tile's adapters in order of first use (the rows are on their way)
+    const int own[1] = {row_adapter(p, row0 + tid)};
+    int ord[1] = {-1};
+    const int n = number_adapters<1>(own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
+    s_ord[tid] = ord[0];
+    if (tid == 0) *s_count = n;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch_dependents();  // after the allocation: the projection allocates too
+  const uint32_t tmem = *tmem_slot;
+  const int n = *s_count;
+  const int u0 = (int)((long long)slice * n / slices), u1 = (int)((long long)(slice + 1) * n / slices);
+  const int per = kShrinkCols / cols;  // adapters of one pass
+  if (warp == 4 && u0 == u1)           // no adapter here: the rows still land before the exit
+    for (int k = 0; k < ST && k < nkb; ++k) {
+      if (elect_one()) mbar_arrive(&full[k]);
+      __syncwarp();
+      if (!warp_wait(&full[k], 0, limit) && lane == 0) atomicExch(failed, 1);
+    }
+  Ring<ST> ring;
+  uint32_t g = 0, pass = 0;  // K blocks and passes before this one
+  for (int u = u0; u < u1; u += per, ++pass) {
+    // (after a failure the passes still meet at their barriers)
+    const int units = u1 - u < per ? u1 - u : per;
+    const int todo = *reinterpret_cast<volatile int*>(failed) ? 0 : nkb;
+    if (warp == 4) {
+      for (int k = 0; k < todo; ++k, ++g, ring.next()) {
+        const int s = ring.s;
+        if (g >= ST && !warp_wait(&empty[s], ring.phase ^ 1, limit)) {
+          if (lane == 0) atomicExch(failed, 1);
+          break;
+        }
+        if (elect_one()) {
+          if (g >= ST || (int)g >= nkb) load_rows(s, k);  // (the first ones were requested above)
+          mbar_expect_tx(&full[s], units * cols * 128);
+          for (int a = 0; a < units; ++a)
+            tma_load_3d(sA + s * kShrinkABytes + a * cols * 128, &amap, &full[s], (kb0 + k) * 64, group * kShrinkRanks,
+                        s_list[u + a], pol);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 5) {
+      const uint32_t idesc = idesc_bf16(128, units * cols);
+      const uint32_t x0 = desc_lo(smem_u32(sX)), a0 = desc_lo(smem_u32(sA));
+      for (int k = 0; k < todo; ++k, ring.next()) {
+        const int s = ring.s;
+        if (!warp_wait(&full[s], ring.phase, limit)) {
+          if (lane == 0) atomicExch(failed, 1);
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t xd = x0 + s * (kShrinkXBytes >> 4), ad = a0 + s * (kShrinkABytes >> 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            umma1_f16<kDesc128, kDesc128>(tmem, xd + 2 * e, ad + 2 * e, idesc, (k | e) != 0);
+          umma_commit(&empty[s]);
+        }
+        __syncwarp();
+      }
+      if (elect_one()) umma_commit(done);
+      __syncwarp();
+    } else {
+      if (!warp_wait(done, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      tc_fence_after();
+      // a row keeps the columns of its own adapter
+      const int ord = s_ord[tid];
+      for (int a = 0; a < units; ++a) {
+        const bool mine = ord == u + a;
+        if (!__any_sync(0xffffffffu, mine)) continue;
+        for (int c = 0; c < cols; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + a * cols + c, r);
+          tmem_wait_ld();
+          if (mine)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(part + tid * kShrinkPitch + c + e) =
+                  make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]),
+                              __uint_as_float(r[e + 3]));
+        }
+      }
+      tc_fence_before();
+    }
+    if (split > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    tc_fence_after();
+    if (warp < 4) {
+      const int t0 = rank * kShrinkRows / split, rows = (rank + 1) * kShrinkRows / split - t0;
+      const uint32_t base = smem_u32(part);
+      const int quads = cols / 4;
+      // four ranks of a row at a time; the parts of all K slices are requested
+      // before the first is added
+      for (int e = tid; e < rows * quads; e += 128) {
+        const int row = t0 + e / quads, c = e % quads * 4, r = group * kShrinkRanks + c, o = s_ord[row];
+        if (o < u || o >= u + units || (r >> 5) >= p.chunks) continue;
+        const int off = row * kShrinkPitch + c;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (split == 1) {
+          v = *reinterpret_cast<const float4*>(part + off);
+        } else {
+          float4 q[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < split) q[k] = ld_dsmem_f32x4(mapa_shared(base, k) + off * 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < split) {
+              v.x += q[k].x;
+              v.y += q[k].y;
+              v.z += q[k].z;
+              v.w += q[k].w;
+            }
+        }
+        const float f = p.scaling ? p.scaling[s_list[o]] : 1.f;
+        const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        float lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
+          lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
+        __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+      }
+    }
+    // the partial sums are read; the next pass's copies may take their place
+    fence_proxy_async_smem();
+    if (split > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) tmem_dealloc(tmem, kShrinkCols);
+  if (tid == 0 && *reinterpret_cast<volatile int*>(failed))
+    record_status(p.status ? p.status : &g_op_status, kStatusGemmFullTimeout);
+}
+
+// ---------------------------------------------------------- shrink, few rows
+// The same for up to 64 rows, which may each bring an adapter of their own:
+// CTAs of 64 rows on mma.sync, whose operands TMA stages, without tensor memory
+// and in little shared memory, so that many share an SM and the projection's
+// CTAs start beside them (64 rows with 64 adapters of rank 16 into 5,248
+// features: 18.6 us with this one in front, 24.3 with the one above).
+constexpr int kFewRows = 64;
+
+// WIDE: one adapter of more than 32 ranks at a time; else adapters that
+// together have up to 32 columns, and a stage more in the same memory.
+template <bool WIDE>
+struct FewShrinkCfg {
+  static constexpr int COLS = WIDE ? 64 : 32;
+  static constexpr int STAGES = WIDE ? 3 : 4;
+  static constexpr int X_BYTES = kFewRows * 128, A_BYTES = COLS * 128;
+  static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
+  static constexpr int PART_BYTES = kFewRows * kShrinkPitch * 4;  // over the stages, between passes
+  static_assert(PART_BYTES <= PIPE_BYTES, "the partial sums fit the pipeline's memory");
+  static constexpr int SMEM = PIPE_BYTES + (2 * 128 + 264) * 4 + 128 + 1024;
+};
+
+DEVI void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DEVI void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr)
+               : "memory");
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(160)
+    lora_shrink_few_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
+                       const LoraParams p) {
+  using C = FewShrinkCfg<WIDE>;
   constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -203,13 +418,11 @@ __global__ void __launch_bounds__(160)
   const bool loader = warp == 4;
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, slices = gridDim.y / groups;
   const int group = blockIdx.y % groups, slice = blockIdx.y / groups;
-  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
-  if ((int)blockIdx.x >= tiles) {  // the CTAs behind the row tiles write the projection's lists
-    if (blockIdx.y == 0 && blockIdx.z == 0 && !loader)
-      write_list(p, ((int)blockIdx.x - tiles) * 256, reinterpret_cast<int*>(smem));
+  if (blockIdx.x == 1) {  // these CTAs write the projection's list
+    if (blockIdx.y == 0 && blockIdx.z == 0 && !loader) write_list(p, 0, reinterpret_cast<int*>(smem));
     return;
   }
-  const int row0 = blockIdx.x * kShrinkRows, split = gridDim.z, rank = blockIdx.z;
+  const int split = gridDim.z, rank = blockIdx.z;
   const int cols = lora_shrink_box(p.rank);  // of one adapter
   const int kblocks = (p.in_features + 63) / 64;
   const int kb0 = rank * kblocks / split, nkb = (rank + 1) * kblocks / split - kb0;
@@ -217,7 +430,7 @@ __global__ void __launch_bounds__(160)
   const uint64_t pol = policy_evict_last();
   auto load_rows = [&](int s, int k) {
     mbar_expect_tx(&full[s], C::X_BYTES);
-    tma_load_2d(sX + s * C::X_BYTES, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
+    tma_load_2d(sX + s * C::X_BYTES, &xmap, &full[s], (kb0 + k) * 64, 0, pol);
   };
   if (loader) {
     if (elect_one()) {
@@ -232,7 +445,7 @@ __global__ void __launch_bounds__(160)
     __syncwarp();
   } else {
     // ---- the tile's adapters in order of first use (the rows are on their way)
-    const int own[1] = {tid < kShrinkRows ? row_adapter(p, row0 + tid) : -1};
+    const int own[1] = {tid < kFewRows ? row_adapter(p, tid) : -1};
     int ord[1] = {-1};
     const int n = number_adapters<1>(own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
     s_ord[tid] = ord[0];
@@ -316,7 +529,7 @@ __global__ void __launch_bounds__(160)
     else
       __syncthreads();
     if (!loader) {
-      const int t0 = rank * kShrinkRows / split, rows = (rank + 1) * kShrinkRows / split - t0;
+      const int t0 = rank * kFewRows / split, rows = (rank + 1) * kFewRows / split - t0;
       const uint32_t base = smem_u32(part);
       const int quads = cols / 4;
       // four ranks of a row at a time; the parts of all K slices are requested
@@ -348,7 +561,7 @@ __global__ void __launch_bounds__(160)
 #pragma unroll
         for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
           lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
-        __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
+        __nv_bfloat16* dst = p.v + ((size_t)row * p.chunks + (r >> 5)) * 64 + (r & 31);
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
       }
@@ -797,27 +1010,12 @@ cudaError_t dispatch_bn(int bn, const LoraMaps& maps, const GemmParams& p, const
 
 namespace {
 
-template <bool WIDE>
-cudaError_t shrink_one(const LoraMaps& maps, const LoraParams& p, dim3 grid, cudaStream_t stream, bool pdl) {
-  constexpr int kSmem = ShrinkCfg<WIDE>::SMEM;
-  auto kern = lora_shrink_kernel<WIDE>;
-  static std::mutex mu;
-  static uint64_t ready = 0;
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!(ready >> dev & 1)) {
-      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-      if (err != cudaSuccess) return err;
-      ready |= uint64_t(1) << dev;
-    }
-  }
+cudaError_t launch_shrink(const void* kern, int smem, int threads, dim3 grid, const LoraMaps& maps, const LoraParams& p,
+                          cudaStream_t stream, bool pdl) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(160, 1, 1);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   cfg.attrs = attrs;
@@ -831,7 +1029,8 @@ cudaError_t shrink_one(const LoraMaps& maps, const LoraParams& p, dim3 grid, cud
     attrs[cfg.numAttrs].val.clusterDim.y = 1;
     attrs[cfg.numAttrs++].val.clusterDim.z = grid.z;
   }
-  return cudaLaunchKernelEx(&cfg, kern, maps.rows, maps.a, p);
+  void* args[] = {const_cast<CUtensorMap*>(&maps.rows), const_cast<CUtensorMap*>(&maps.a), const_cast<LoraParams*>(&p)};
+  return cudaLaunchKernelExC(&cfg, kern, args);
 }
 
 }  // namespace
@@ -840,19 +1039,44 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
       p.index_div < 1 || !p.lists)
     return cudaErrorInvalidValue;
-  // One wave of CTAs: few rows (single rows of many requests) may each bring
-  // an adapter, so their adapters are spread first; many rows share a few, and
-  // there only K is split.
-  const bool wide = p.rank > 32;
-  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows, groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks;
-  const int kblocks = (p.in_features + 63) / 64, per = (wide ? 64 : 32) / lora_shrink_box(p.rank);
-  const int room = std::max(1, kShrinkPerSm * sm_count / (tiles * groups));
-  const int most = std::min(p.slots, std::min(p.rows, kShrinkRows));
-  const int slices = p.rows <= 256 ? std::min(room, (most + per - 1) / per) : 1;
+  constexpr int kWide = FewShrinkCfg<true>::SMEM, kSlim = FewShrinkCfg<false>::SMEM;
+  static std::mutex mu;
+  static uint64_t ready = 0;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!(ready >> dev & 1)) {
+      const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+      err = cudaFuncSetAttribute(lora_shrink_kernel, attr, kShrinkSmem);
+      if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_shrink_few_kernel<true>, attr, kWide);
+      if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_shrink_few_kernel<false>, attr, kSlim);
+      if (err != cudaSuccess) return err;
+      ready |= uint64_t(1) << dev;
+    }
+  }
+  const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, kblocks = (p.in_features + 63) / 64;
+  if (lora_shrink_rows(p.rows) == kFewRows) {
+    // The adapters are spread first, then K, up to three CTAs per SM.
+    const bool wide = p.rank > 32;
+    const int per = (wide ? 64 : 32) / lora_shrink_box(p.rank), room = std::max(1, 3 * sm_count / groups);
+    const int slices = std::min(room, (std::min(p.slots, p.rows) + per - 1) / per);
+    int split = 1;
+    while (split < 8 && 2 * split <= kblocks && 2 * split * slices <= room) split *= 2;
+    const dim3 grid(2, groups * slices, split);
+    return wide ? launch_shrink((const void*)lora_shrink_few_kernel<true>, kWide, 160, grid, maps, p, stream, pdl)
+                : launch_shrink((const void*)lora_shrink_few_kernel<false>, kSlim, 160, grid, maps, p, stream, pdl);
+  }
+  // One CTA per SM: K is split until they are in use (two K blocks at least
+  // each), then the adapters, of which single rows of many requests bring many.
+  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
+  const int room = std::max(1, sm_count / (tiles * groups));
   int split = 1;
-  while (split < 8 && 2 * split <= kblocks && 2 * split * slices <= room) split *= 2;
-  const dim3 grid(tiles + (p.rows + 255) / 256, groups * slices, split);
-  return wide ? shrink_one<true>(maps, p, grid, stream, pdl) : shrink_one<false>(maps, p, grid, stream, pdl);
+  while (split < 8 && 4 * split <= kblocks && 2 * split <= room) split *= 2;
+  const int slices = std::max(1, std::min(room / split, std::min(p.slots, std::min(p.rows, kShrinkRows))));
+  return launch_shrink((const void*)lora_shrink_kernel, kShrinkSmem, 192,
+                       dim3(tiles + (p.rows + 255) / 256, groups * slices, split), maps, p, stream, pdl);
 }
 
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,

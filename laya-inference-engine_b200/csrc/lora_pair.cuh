@@ -230,16 +230,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     const uint32_t full0 = mapa_shared(smem_u32(full), 0);
     uint32_t g = 0;
     Ring<ST> ring;
-    bool waited = false, ok = true;
-    ListHead head{};
+    bool ok = true;
     auto stage_free = [&] { return g < ST || warp_wait(&empty[ring.s], ring.phase ^ 1, limit); };
-    for (int t = pair; t < tiles && ok; t += pairs) {
-      const int tm = t % tiles_m, tn = t / tiles_m;
-      const int m0 = tm * 256 + (int)rank * 128, n0 = tn * BNF + (int)rank * (BNF / 2);
-      if (waited) head = head_of(tm);  // on its way during the K blocks
+    auto k_blocks = [&](int t) {
+      const int m0 = t % tiles_m * 256 + (int)rank * 128, n0 = t / tiles_m * BNF + (int)rank * (BNF / 2);
       for (int kb = 0; kb < p.kblocks; ++kb, ++g, ring.next()) {
         const int s = ring.s;
-        if (!(ok = stage_free())) break;
+        if (!(ok = stage_free())) return;
         if (elect_one()) {
           if (leader) mbar_expect_tx(&full[s], 2 * C::STAGE_BYTES);
           tma2_load_2d(sA + s * C::A_BYTES, &xmap, full0 + s * 8, kb * C::K_ELEMS, m0, pol_x);
@@ -247,16 +244,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         }
         __syncwarp();
       }
-      if (!ok) break;
-      if (!waited) {
-        griddep_wait();
-        waited = true;
-        head = head_of(tm);
-      }
+    };
+    auto adapter_blocks = [&](int t, const ListHead& head) {
+      const int tm = t % tiles_m;
+      const int m0 = tm * 256 + (int)rank * 128, n0 = t / tiles_m * BNF + (int)rank * (BNF / 2);
       const int nb = head.count * lp.chunks;
       for (int b = 0; b < nb; ++b, ++g, ring.next()) {
         const int s = ring.s, c = b % lp.chunks, slot = slot_of(head, tm, b / lp.chunks);
-        if (!(ok = stage_free())) break;
+        if (!(ok = stage_free())) return;
         if (elect_one()) {
           if (leader) mbar_expect_tx(&full[s], BNF * 64);
           tma2_load_3d(sB + s * C::B_BYTES, &bmap, full0 + s * 8, c * 32, n0, slot, pol_x);
@@ -265,6 +260,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         }
         __syncwarp();
       }
+    };
+    // Both accumulators take their K blocks before the first adapter block has
+    // to wait for the shrink.
+    const int t1 = pair + pairs < tiles ? pair + pairs : -1;
+    k_blocks(pair);
+    if (ok && t1 >= 0) k_blocks(t1);
+    griddep_wait();
+    if (ok) adapter_blocks(pair, head_of(pair % tiles_m));
+    if (ok && t1 >= 0) adapter_blocks(t1, head_of(t1 % tiles_m));
+    for (int t = pair + 2 * pairs; t < tiles && ok; t += pairs) {
+      const ListHead head = head_of(t % tiles_m);  // on its way during the K blocks
+      k_blocks(t);
+      if (ok) adapter_blocks(t, head);
     }
     if (!ok && lane == 0) give_up(kStatusGemmEmptyTimeout);
     // every stage's last release, so that none is in flight at the exit
@@ -280,21 +288,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     const uint32_t idesc = KIND == kKindBf16 ? idesc_bf16(256, BNF) : idesc_e4m3(256, BNF);
     const uint32_t idesc2 = idesc_bf16(256, BNF);
     const uint32_t a0 = desc_lo(smem_u32(sA)), b0 = desc_lo(smem_u32(sB));
-    uint32_t vphase = 0, n = 0;
+    uint32_t vphase = 0;
     Ring<ST> ring;
-    bool waited = false, ok = true;
-    for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-      const int tm = t % tiles_m, buf = n & 1;
-      const uint32_t acc = tmem + buf * 256, acc2 = acc + (KIND == kKindFp8 ? BNF : 0);
-      int nb = waited ? blocks_of(tm) : 0;  // on its way during the K blocks
-      if (n >= 2 && !warp_wait(&acc_empty[buf], ((n >> 1) - 1) & 1, limit)) {
-        ok = false;
-        break;
-      }
+    bool ok = true;
+    // n: the tile's place among the pair's tiles
+    auto k_blocks = [&](uint32_t n) {
+      const uint32_t acc = tmem + (n & 1) * 256;
+      if (n >= 2 && !(ok = warp_wait(&acc_empty[n & 1], ((n >> 1) - 1) & 1, limit))) return;
       tc_fence_after();
       for (int kb = 0; kb < p.kblocks; ++kb, ring.next()) {
         const int s = ring.s;
-        if (!(ok = warp_wait(&full[s], ring.phase, limit))) break;
+        if (!(ok = warp_wait(&full[s], ring.phase, limit))) return;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t ad = a0 + s * (C::A_BYTES >> 4), bd = b0 + s * (C::B_BYTES >> 4);
@@ -309,17 +313,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         }
         __syncwarp();
       }
-      if (!ok) break;
-      if (!waited) {
-        griddep_wait();
-        waited = true;
-        nb = blocks_of(tm);
-      }
+    };
+    auto adapter_blocks = [&](uint32_t n, int nb) {
+      const uint32_t acc2 = tmem + (n & 1) * 256 + (KIND == kKindFp8 ? BNF : 0);
       for (int b = 0; b < nb; ++b, ring.next()) {
         const int s = ring.s;
-        if (!(ok = warp_wait(&full[s], ring.phase, limit)) ||
-            !(ok = warp_wait(&vfull[s], (vphase >> s) & 1, limit)))
-          break;
+        if (!(ok = warp_wait(&full[s], ring.phase, limit)) || !(ok = warp_wait(&vfull[s], (vphase >> s) & 1, limit)))
+          return;
         vphase ^= 1u << s;
         tc_fence_after();
         if (elect_one()) {
@@ -334,8 +334,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         }
         __syncwarp();
       }
-      if (ok && elect_one()) umma2_commit(&acc_full[buf]);
+      if (elect_one()) umma2_commit(&acc_full[n & 1]);
       __syncwarp();
+    };
+    const int t1 = pair + pairs < tiles ? pair + pairs : -1;
+    k_blocks(0);
+    if (ok && t1 >= 0) k_blocks(1);
+    griddep_wait();
+    if (ok) adapter_blocks(0, blocks_of(pair % tiles_m));
+    if (ok && t1 >= 0) adapter_blocks(1, blocks_of(t1 % tiles_m));
+    uint32_t n = 2;
+    for (int t = pair + 2 * pairs; t < tiles && ok; t += pairs, ++n) {
+      const int nb = blocks_of(t % tiles_m);  // on its way during the K blocks
+      k_blocks(n);
+      if (ok) adapter_blocks(n, nb);
     }
     if (!ok && lane == 0) give_up(kStatusGemmFullTimeout);
   } else if (warp == 2 || warp == 3) {
@@ -348,7 +360,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       const int tm = t % tiles_m, m0 = tm * 256 + (int)rank * 128;
       const ListHead head = head_of(tm);
       const int nb = head.count * lp.chunks;
-      g += p.kblocks;
+      // the ring positions of the K blocks before: two tiles' before the first
+      if (t == pair)
+        g = (pair + pairs < tiles ? 2 : 1) * p.kblocks;
+      else if (t >= pair + 2 * pairs)
+        g += p.kblocks;
       const int own0 = row_adapter(lp, m0 + r0), own1 = row_adapter(lp, m0 + r0 + 32);
       for (int b = 0; b < nb; ++b, ++g) {
         const int s = g % ST, slot = slot_of(head, tm, b / lp.chunks);
