@@ -4,7 +4,9 @@
 
 Every .cu under csrc/ is compiled to an object in _build/ (in parallel, only
 when its sources changed) and linked into laya_b200/liblaya_b200.so.  nvcc
-cross-compiles without a GPU.
+cross-compiles without a GPU.  csrc/torch_ops.cpp becomes laya_b200/_torch_ops.so
+(the torch calls of laya_b200/ops.py), linked to that library, when torch is
+installed; the engine itself does not need it.
 """
 import argparse
 import concurrent.futures as cf
@@ -12,11 +14,13 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "laya_b200" / "liblaya_b200.so"
+TORCH_OUT = HERE / "laya_b200" / "_torch_ops.so"
 BUILD = HERE / "_build"
 INCLUDE = HERE.parent / "include"
 
@@ -72,7 +76,39 @@ def build(force=False, verbose=False):
     os.replace(tmp, OUT)
     if verbose:
         print(f"built {OUT}")
+    if _build_torch_ops(force) and verbose:
+        print(f"built {TORCH_OUT}")
     return OUT
+
+
+def _build_torch_ops(force):
+    try:
+        import torch
+    except ImportError:
+        return False
+    src = CSRC / "torch_ops.cpp"
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+             f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{cuda}/include",
+             f"-I{sysconfig.get_paths()['include']}"]
+    # the object by its path: a dependency of the name that lies beside it at run time
+    link = ["-shared", f"-L{OUT.parent}", f"-l:{OUT.name}", "-Wl,-rpath,$ORIGIN", f"-L{root}/lib", "-lc10", "-lc10_cuda",
+            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    h = hashlib.sha256(" ".join(flags + link + [torch.__version__]).encode())
+    h.update(src.read_bytes())
+    h.update((INCLUDE / "laya_b200.h").read_bytes())
+    stamp = BUILD / "torch_ops.stamp"
+    if not force and TORCH_OUT.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
+        return True
+    tmp = TORCH_OUT.with_suffix(".so.tmp")
+    r = subprocess.run(["g++", *flags, str(src), "-o", str(tmp), *link], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{r.stderr}")
+    os.replace(tmp, TORCH_OUT)
+    stamp.write_text(h.hexdigest())
+    return True
 
 
 if __name__ == "__main__":

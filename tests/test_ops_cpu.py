@@ -117,12 +117,3 @@ def test_stack_adapters():
     with pytest.raises(ValueError):
         ops.stack_adapters([(torch.ones(10, 16), torch.ones(8, 10), 1.0)], rank=8, device="cpu")
 
-
-def test_packed_arguments_have_the_c_layout():
-    """ops packs the argument blocks itself: same size and field offsets as the
-    structures of the header's binding."""
-    for packed, cls in ((ops._RMS_ARGS, _lib.RmsNormArgs), (ops._LORA_ARGS, _lib.LoraArgs)):
-        assert packed.size == ctypes.sizeof(cls)
-        values = [1.5 if kind is ctypes.c_float else i + 1 for i, (_, kind) in enumerate(cls._fields_)]
-        got = cls.from_buffer_copy(packed.pack(*values))
-        assert [getattr(got, name) for name, _ in cls._fields_] == values
