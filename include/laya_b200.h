@@ -78,10 +78,34 @@ LAYA_B200_API int laya_b200_build_token_tables(laya_b200_engine* e);
  * caller, calls on different lanes may overlap. */
 LAYA_B200_API int laya_b200_create_lane(laya_b200_engine* parent, laya_b200_engine** lane);
 
+/* Adapters (no counterpart in the reference): low-rank additions to the
+ * encoder projections, scaling (x A^T) B^T beside x W^T, chosen per question of
+ * a batch.  enable_adapters reserves `slots` of them, each of rank up to
+ * max_rank (rounded up to a multiple of 8), once, after finalize and before
+ * lanes are created; bf16 and FP8 engines (the adapters stay bf16).  They cost
+ * slots * rank * 2 bytes per row and column of every projection (0.9 MB per
+ * slot and rank for the Laya shape), shared with the lanes. */
+LAYA_B200_API int laya_b200_enable_adapters(laya_b200_engine* e, int slots, int max_rank);
+
+/* Upload one projection's part of the adapter in `slot`: name "enc.{i}.wqkv",
+ * "wo", "wi" or "wo2", a [rank][in] and b [out][rank] host bf16 bit patterns
+ * (b's rows as set_weight takes the weight's), which have to be finite.  A
+ * projection that was not set adds nothing.  No run on the engine or its lanes
+ * may be in progress; the same holds for clear_adapter, which zeroes a slot. */
+LAYA_B200_API int laya_b200_set_adapter(laya_b200_engine* e, int slot, const char* name, int rank, const void* a,
+                                        const void* b, float scaling);
+LAYA_B200_API int laya_b200_clear_adapter(laya_b200_engine* e, int slot);
+
 /* Capture the forward for one padded shape into CUDA graphs (the analogue
  * of BlackwellEngine._slot, engine.py:161-187).  `unmasked` mirrors the
  * graph key's flag (engine.py:132-138); results do not depend on it. */
 LAYA_B200_API int laya_b200_capture(laya_b200_engine* e, int batch, int seq, int options, int unmasked, int* slot);
+
+/* The same for batches whose questions select adapters.  Such a forward runs
+ * every encoder projection with adapters; it uses neither the batch-1 fusions
+ * nor the token tables. */
+LAYA_B200_API int laya_b200_capture_adapters(laya_b200_engine* e, int batch, int seq, int options, int unmasked,
+                                             int* slot);
 
 /* Drop a captured slot (LRU eviction, engine.py:167-169). */
 LAYA_B200_API int laya_b200_release(laya_b200_engine* e, int slot);
@@ -96,6 +120,13 @@ LAYA_B200_API int laya_b200_release(laya_b200_engine* e, int slot);
 LAYA_B200_API int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const int64_t* attention_mask,
                   const int64_t* marker_pos, const uint8_t* marker_mask, const int64_t* qtype, float* logits,
                   float* act);
+
+/* laya_b200_run on a slot of capture_adapters: adapter [batch] int32, the
+ * adapter slot of each question or -1 (NULL: none for any). */
+LAYA_B200_API int laya_b200_run_adapters(laya_b200_engine* e, int slot, const int64_t* input_ids,
+                                         const int64_t* attention_mask, const int64_t* marker_pos,
+                                         const uint8_t* marker_mask, const int64_t* qtype, const int32_t* adapter,
+                                         float* logits, float* act);
 
 /* Measurement helper: replay the kernels-only graph `iterations` times back
  * to back on the inputs already resident on the device (from the last run)

@@ -135,6 +135,7 @@ struct Proj {
 
 struct Shape {
   int b, s, k, unmasked;
+  int adapters = 0;  // questions select an adapter
 };
 
 // Capacity of the split-K partial scratch (floats): larger reductions fall
@@ -144,7 +145,7 @@ constexpr size_t kPartialFloats = (size_t)16 * 1024 * 1024;
 // Compact per-shape layout of the int32 input words and fp32 output words, so
 // each step copies only what the shape needs.
 struct IoLayout {
-  size_t ids, valid, qtype, mmask, selsrc, selpos, score, words;
+  size_t ids, valid, qtype, mmask, selsrc, selpos, score, adapter, words;
   size_t logits, act, out_words;
 };
 
@@ -159,6 +160,8 @@ IoLayout io_layout(const Shape& sh) {
   L.selsrc = o; o += R;
   L.selpos = o; o += R;
   L.score = o; o += BK;
+  L.adapter = o;
+  if (sh.adapters) o += b;
   L.words = o;
   L.logits = 0;
   L.act = BK;
@@ -177,6 +180,17 @@ struct Slot {
   bool live = false;
 };
 
+// Encoder projections that adapters extend, in this order per layer.
+constexpr const char* kAdapted[4] = {"wqkv", "wo", "wi", "wo2"};
+
+// The adapter slots of one projection: A [slots][rank][K], B [slots][N][rank]
+// (rows as the packed weight has them), scaling [slots].
+struct AdapterSet {
+  __nv_bfloat16* a = nullptr;
+  __nv_bfloat16* b = nullptr;
+  float* scaling = nullptr;
+};
+
 // Weight memory shared by an engine and its lanes; freed with the last one.
 struct WeightShare {
   std::mutex mu;
@@ -185,6 +199,7 @@ struct WeightShare {
   uint8_t* qarena = nullptr;
   float* table_h = nullptr;             // token tables (optional)
   __nv_bfloat16* table_qkv = nullptr;
+  uint8_t* adapters = nullptr;          // adapter slots (optional)
 };
 
 }  // namespace
@@ -209,6 +224,12 @@ struct laya_b200_engine {
   // [vocab][3d] (before the rotary embedding), or null
   float* table_h = nullptr;
   __nv_bfloat16* table_qkv = nullptr;
+  // adapter slots: [layer * 4 + projection], or empty
+  std::vector<AdapterSet> adapters;
+  int adapter_slots = 0, adapter_rank = 0;
+  uint8_t* lora_arena = nullptr;    // V rows and adapter lists of one projection
+  __nv_bfloat16* lora_v = nullptr;
+  int* lora_lists = nullptr;
 
   // activations
   uint8_t* aarena = nullptr;
@@ -576,6 +597,75 @@ struct Fwd {
     return rotated;
   }
 
+  // Encoder projection `which` (kAdapted) of layer i with the adapters of the
+  // questions: x the bf16 rows, codes / x_scale the FP8 operand of the shared
+  // projection (FP8 engines).
+  void gemm_lora(const Proj& w, int i, int which, const __nv_bfloat16* x, const uint8_t* codes, const float* x_scale,
+                 int M, int s, const int* adapter, int epi, __nv_bfloat16* out, int ldo, float* resid,
+                 const float* rope_cos = nullptr, const float* rope_sin = nullptr) {
+    if (!on(kCatGemm)) return;
+    const AdapterSet& ad = e->adapters[i * 4 + which];
+    const int esize = w.kind == kKindBf16 ? 2 : 1, chunks = (e->adapter_rank + 31) / 32;
+    GemmParams p{};
+    p.M = M;
+    p.N = w.N;
+    p.K = w.K;
+    p.kblocks = (w.K + gemm_k_elems(w.kind) - 1) / gemm_k_elems(w.kind);
+    p.epilogue = epi;
+    p.out = out;
+    p.ldo = ldo;
+    p.resid = resid;
+    p.ldr = e->cfg.hidden;
+    p.a_scale = x_scale;
+    p.w_scale = w.w_scale;
+    p.status = e->status_dev;
+    if (rope_cos) {
+      p.rope_cos = rope_cos;
+      p.rope_sin = rope_sin;
+      p.rope_seq = s;
+      p.rope_cols = 2 * (w.N / 3);
+    }
+    LoraParams lp{};
+    lp.rows = M;
+    lp.in_features = w.K;
+    lp.slots = e->adapter_slots;
+    lp.rank = e->adapter_rank;
+    lp.chunks = chunks;
+    lp.index = adapter;
+    lp.index_div = s;
+    lp.x = x;
+    lp.ldx = w.K;
+    lp.a = ad.a;
+    lp.scaling = ad.scaling;
+    lp.v = e->lora_v;
+    lp.lists = e->lora_lists;
+    lp.status = e->status_dev;
+    const int bnf = lora_pair_plan(w.kind, M, w.N, e->sm_count);
+    int bn = 128, split = 1;
+    if (!bnf) {
+      lora_few_plan(M, w.N, p.kblocks, e->sm_count, &bn, &split);
+      if (split > 1 && (size_t)(w.N / 128) * split * bn * 128 <= kPartialFloats) p.partials = e->gpart;
+    }
+    p.tma_epilogue = bnf ? 1 : 0;
+    const int wbox = bnf ? bnf / 2 : 128;
+    LoraMaps maps{};
+    bool ok = rows_map(&maps.rows, x, M, w.K, w.K, 2, lora_shrink_rows(M)) &&
+              slots_map(&maps.a, ad.a, lp.slots, lp.rank, w.K, 64, lora_shrink_box(lp.rank),
+                        CU_TENSOR_MAP_SWIZZLE_128B) &&
+              rows_map(&maps.w, w.w, w.N, w.K, w.K, esize, wbox) &&
+              rows_map(&maps.x, codes ? (const void*)codes : (const void*)x, M, w.K, w.K, esize, bn) &&
+              slots_map(&maps.b, ad.b, lp.slots, w.N, lp.rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (ok && bnf) {
+      ok = rows_map(&maps.v, lp.v, M, chunks * 64, chunks * 64, 2, 128) &&
+           (epi == kEpiResidual ? rows_map(&maps.out, resid, M, p.ldr, p.ldr, 4, 32)
+                                : rows_map(&maps.out, out, M, epi == kEpiGeglu ? w.N / 2 : w.N, ldo, 2, 32));
+    }
+    if (!ok) fail("tensor map rejected for a %dx%d projection with adapters", M, w.N);
+    count(launch_lora_shrink(maps, lp, e->sm_count, st, pdl()), "adapter shrink launch");
+    count(bnf ? launch_lora_pairs(w.kind, maps, p, lp, bnf, st) : launch_lora_gemm(w.kind, maps, p, lp, bn, split, st),
+          "adapter projection launch");
+  }
+
   // Output tensor map of the TMA epilogue (unsplit tiles).
   static int output_map(CUtensorMap* m, const GemmParams& p, int bn) {
     if (p.epilogue == kEpiResidual) return make_plain_map(m, p.resid, p.M, p.ldr, 4, 128, bn) ? 1 : 0;
@@ -645,9 +735,14 @@ struct Fwd {
     const int* selsrc = in + L.selsrc;
     const int* selpos = in + L.selpos;
     const int* score_rows = in + L.score;
+    // Questions with adapters: every encoder projection adds theirs.  The
+    // batch-1 fusions and the token tables (whose layer-0 rows hold none) are
+    // left out, and the norms keep the bf16 rows that the adapters read.
+    const bool ad = sh.adapters != 0;
+    const int* adapter = in + L.adapter;
 
     // Token tables: one gather gives h and the rotated layer-0 qkv.
-    const bool tables = E.table_h != nullptr && c.layers > 0;
+    const bool tables = E.table_h != nullptr && c.layers > 0 && !ad;
     if (tables && on(kCatRows)) {
       TokenGatherParams g{};
       g.rows = T;
@@ -682,6 +777,7 @@ struct Fwd {
       } else {
         p.out_bf16 = E.n;
       }
+      if (ad) p.out_bf16 = E.n;
       norm(p);
     }
     // LayerNorm feeding the encoder projection w: bf16, e4m3 + row scales, or
@@ -700,6 +796,7 @@ struct Fwd {
       } else {
         p.out_bf16 = E.n;
       }
+      if (ad) p.out_bf16 = E.n;
       return p;
     };
     // final_norm(h + pending) + type_emb(qtype) (model.py:102-104), fused with
@@ -726,7 +823,7 @@ struct Fwd {
     // One short sequence in bf16 (the latency path): attention runs inside the
     // Wo projection, and attn_norm / mlp_norm inside the QKV / Wi projections,
     // from row statistics written by the residual projection before them.
-    const bool short_bf16 = !fp8 && !nv4 && b == 1 && c.layers > 0 && ln_plan(E.wqkv[0], T) &&
+    const bool short_bf16 = !fp8 && !nv4 && !ad && b == 1 && c.layers > 0 && ln_plan(E.wqkv[0], T) &&
                             ln_plan(E.wi[0], T);
     for (int i = 0; i < c.layers; ++i) {
       const std::string pre = "enc." + std::to_string(i) + ".";
@@ -738,7 +835,10 @@ struct Fwd {
       bool rotated = true;
       if (tables && i == 0) {
         // layer-0 qkv came from the token tables
-      } else if (short_bf16 && i > 0)
+      } else if (ad)
+        gemm_lora(E.wqkv[i], i, 0, E.n, fp8 ? E.n8 : nullptr, E.n8s, T, s, adapter, kEpiStore, E.qkv, 3 * d, nullptr, rc,
+                  rs);
+      else if (short_bf16 && i > 0)
         gemm_ln(E.wqkv[i], wptr<float>(e, pre + "attn_norm.w"), T, kEpiStore, E.qkv, 3 * d, rc, rs, s);
       else
         rotated = nv4 ? gemm_nv4(E.wqkv[i], E.n, T, kEpiStore, E.qkv, 3 * d, nullptr, 0, rc, rs, s, true)
@@ -755,7 +855,7 @@ struct Fwd {
       a.window = glob ? -1 : c.local_window;
       a.out = E.attn;
       a.ld_out = d;
-      const bool fused = !fp8 && !nv4 && b == 1 && gemm_attn(E.wo[i], a, T);
+      const bool fused = !fp8 && !nv4 && !ad && b == 1 && gemm_attn(E.wo[i], a, T);
       if (short_bf16 && !fused) fail("batch-1 plan: the attention projection did not fuse");
       if (!fused) {
         attention(a, b, c.heads);
@@ -768,7 +868,9 @@ struct Fwd {
           q.scale = E.a8s;
           count(launch_quant_fp8(q, st, pdl()), "quant launch");
         }
-        if (nv4)
+        if (ad)
+          gemm_lora(E.wo[i], i, 1, E.attn, fp8 ? E.a8 : nullptr, E.a8s, T, s, adapter, kEpiResidual, nullptr, 0, E.h);
+        else if (nv4)
           gemm_nv4(E.wo[i], E.attn, T, kEpiResidual, nullptr, 0, E.h, d);
         else
           gemm(E.wo[i], fp8 ? (const void*)E.a8 : (const void*)E.attn, E.a8s, T, kEpiResidual, nullptr, 0, E.h, d);
@@ -777,7 +879,9 @@ struct Fwd {
         gemm_ln(E.wi[i], wptr<float>(e, pre + "mlp_norm.w"), T, kEpiGeglu, E.g, I);
       else {
         norm(enc_norm(pre + "mlp_norm.w", E.wi[i]));
-        if (nv4)
+        if (ad)
+          gemm_lora(E.wi[i], i, 2, E.n, fp8 ? E.n8 : nullptr, E.n8s, T, s, adapter, kEpiGeglu, E.g, I, nullptr);
+        else if (nv4)
           gemm_nv4(E.wi[i], E.n, T, kEpiGeglu, E.g, I, nullptr, 0, nullptr, nullptr, 0, true);
         else
           gemm(E.wi[i], fp8 ? (const void*)E.n8 : (const void*)E.n, E.n8s, T, kEpiGeglu, E.g, I, nullptr, 0);
@@ -792,7 +896,9 @@ struct Fwd {
         count(launch_quant_fp8(q, st, pdl()), "quant launch");
       }
       const bool last = i + 1 == c.layers;
-      if (nv4)
+      if (ad)
+        gemm_lora(E.wo2[i], i, 3, E.g, fp8 ? E.g8 : nullptr, E.g8s, T, s, adapter, kEpiResidual, nullptr, 0, E.h);
+      else if (nv4)
         gemm_nv4(E.wo2[i], E.g, T, kEpiResidual, nullptr, 0, E.h, d);
       else
         gemm(E.wo2[i], fp8 ? (const void*)E.g8 : (const void*)E.g, E.g8s, T, kEpiResidual, nullptr, 0, E.h, d,
@@ -1031,7 +1137,7 @@ void alloc_runtime(laya_b200_engine* e) {
   ck(cudaMemcpy(e->lcos, cs.data(), cs.size() * 4, cudaMemcpyHostToDevice), "rope upload");
   ck(cudaMemcpy(e->lsin, sn.data(), sn.size() * 4, cudaMemcpyHostToDevice), "rope upload");
   // I/O staging capacity: the layout of the largest shape
-  const IoLayout cap = io_layout(Shape{c.max_batch, c.max_len, c.max_options, 0});
+  const IoLayout cap = io_layout(Shape{c.max_batch, c.max_len, c.max_options, 0, 1});
   e->in_words = cap.words;
   e->out_words = cap.out_words;
   ck(cudaMalloc(&e->d_in, e->in_words * 4), "input buffer");
@@ -1042,6 +1148,16 @@ void alloc_runtime(laya_b200_engine* e) {
   ck(cudaHostAlloc(&e->status_host, 64, cudaHostAllocMapped), "status word");
   memset(e->status_host, 0, 64);
   ck(cudaHostGetDevicePointer((void**)&e->status_dev, e->status_host, 0), "status pointer");
+}
+
+// V rows and adapter lists of one projection (the largest batch).
+void alloc_lora(laya_b200_engine* e) {
+  const size_t T = (size_t)e->cfg.max_batch * e->cfg.max_len;
+  const size_t v = align_up(T * ((e->adapter_rank + 31) / 32) * 128, 1024);
+  const size_t lists = (T + 255) / 256 * kLoraListInts * sizeof(int);
+  ck(cudaMalloc(&e->lora_arena, v + lists), "adapter activations");
+  e->lora_v = reinterpret_cast<__nv_bfloat16*>(e->lora_arena);
+  e->lora_lists = reinterpret_cast<int*>(e->lora_arena + v);
 }
 
 extern "C" {
@@ -1135,8 +1251,12 @@ int laya_b200_create_lane(laya_b200_engine* parent, laya_b200_engine** out) {
     e->sc_fc1 = parent->sc_fc1;
     e->table_h = parent->table_h;
     e->table_qkv = parent->table_qkv;
+    e->adapters = parent->adapters;
+    e->adapter_slots = parent->adapter_slots;
+    e->adapter_rank = parent->adapter_rank;
     e->finalized = true;
     alloc_runtime(e.get());
+    if (e->adapter_slots) alloc_lora(e.get());
   } catch (const Error& err) {
     g_create_error = err.msg;
     laya_b200_destroy(e.release());
@@ -1186,6 +1306,115 @@ int laya_b200_build_token_tables(laya_b200_engine* e) {
     e->table_h = w->table_h;
     e->table_qkv = w->table_qkv;
     e->inputs_slot = -1;  // the staging buffers were used for the tables
+  });
+}
+
+int laya_b200_enable_adapters(laya_b200_engine* e, int slots, int max_rank) {
+  return guard(e, [&] {
+    if (!e->finalized) fail("finalize the weights before enabling adapters");
+    if (e->precision == LAYA_B200_NVFP4) fail("adapters run beside bf16 and FP8 weights, not NVFP4");
+    if (e->adapter_slots) fail("adapters are already enabled");
+    if (slots < 1 || slots > 4096) fail("adapter slots must be in [1, 4096]");
+    if (max_rank < 1 || max_rank > kLoraMaxRank) fail("max_rank must be in [1, %d]", kLoraMaxRank);
+    if (e->cfg.layers < 1) fail("adapters need an encoder layer");
+    {
+      std::lock_guard<std::mutex> lock(e->weights->mu);
+      if (e->weights->refs > 1) fail("enable adapters before creating lanes");
+    }
+    const int rank = (max_rank + 7) / 8 * 8;
+    std::vector<AdapterSet> sets;
+    size_t off = 0;
+    auto place = [&](size_t bytes) {
+      const size_t at = off;
+      off = align_up(off + bytes, 256);
+      return at;
+    };
+    std::vector<size_t> at;
+    for (int i = 0; i < e->cfg.layers; ++i)
+      for (const char* nm : kAdapted) {
+        const ParamInfo& pi = e->params.at("enc." + std::to_string(i) + "." + nm);
+        at.push_back(place((size_t)slots * rank * pi.cols * 2));
+        at.push_back(place((size_t)slots * rank * pi.rows * 2));
+        at.push_back(place((size_t)slots * 4));
+      }
+    ck(cudaMalloc(&e->weights->adapters, off), "adapter slots");
+    uint8_t* base = e->weights->adapters;
+    try {
+      ck(cudaMemset(base, 0, off), "adapter slots");
+      e->adapter_rank = rank;
+      alloc_lora(e);
+    } catch (...) {
+      cudaFree(base);
+      e->weights->adapters = nullptr;
+      e->adapter_rank = 0;
+      throw;
+    }
+    for (size_t j = 0; j < at.size(); j += 3)
+      sets.push_back(AdapterSet{reinterpret_cast<__nv_bfloat16*>(base + at[j]),
+                                reinterpret_cast<__nv_bfloat16*>(base + at[j + 1]),
+                                reinterpret_cast<float*>(base + at[j + 2])});
+    e->adapters = sets;
+    e->adapter_slots = slots;
+  });
+}
+
+int laya_b200_set_adapter(laya_b200_engine* e, int slot, const char* name, int rank, const void* a, const void* b,
+                          float scaling) {
+  return guard(e, [&] {
+    if (!e->adapter_slots) fail("adapters are not enabled");
+    if (slot < 0 || slot >= e->adapter_slots) fail("adapter slot %d outside [0, %d)", slot, e->adapter_slots);
+    if (!name || !a || !b) fail("null argument");
+    if (rank < 1 || rank > e->adapter_rank) fail("adapter rank %d outside [1, %d]", rank, e->adapter_rank);
+    if (!std::isfinite(scaling)) fail("adapter scaling is not finite");
+    const std::string n(name);
+    int index = -1;
+    for (int i = 0; i < e->cfg.layers && index < 0; ++i)
+      for (int w = 0; w < 4; ++w)
+        if (n == "enc." + std::to_string(i) + "." + kAdapted[w]) index = i * 4 + w;
+    if (index < 0) fail("no adapted projection %s", name);
+    const ParamInfo& pi = e->params.at(n);
+    const int K = pi.cols, N = pi.rows, R = e->adapter_rank, I = e->cfg.intermediate;
+    const uint16_t* ha = static_cast<const uint16_t*>(a);
+    const uint16_t* hb = static_cast<const uint16_t*>(b);
+    // the rows of a tile share matrix instructions: a value that is not finite
+    // would reach other questions
+    auto finite = [](const uint16_t* v, size_t count) {
+      for (size_t i = 0; i < count; ++i)
+        if ((v[i] & 0x7F80) == 0x7F80) return false;
+      return true;
+    };
+    if (!finite(ha, (size_t)rank * K) || !finite(hb, (size_t)N * rank)) fail("adapter %s contains NaN or infinity", name);
+    std::vector<uint16_t> pa((size_t)R * K, 0), pb((size_t)N * R, 0);
+    memcpy(pa.data(), ha, (size_t)rank * K * 2);
+    const bool is_wi = index % 4 == 2;
+    for (int r = 0; r < N; ++r) {
+      // Wi's rows are stored interleaved (set_weight): row r of the packed
+      // matrix is act row j or gate row j of block t
+      const int t = r / 128, j = r % 128;
+      const int src = !is_wi ? r : j < 64 ? 64 * t + j : I + 64 * t + j - 64;
+      memcpy(pb.data() + (size_t)r * R, hb + (size_t)src * rank, (size_t)rank * 2);
+    }
+    const AdapterSet& ad = e->adapters[index];
+    ck(cudaMemcpy(ad.a + (size_t)slot * R * K, pa.data(), pa.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
+    ck(cudaMemcpy(ad.b + (size_t)slot * N * R, pb.data(), pb.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
+    ck(cudaMemcpy(ad.scaling + slot, &scaling, 4, cudaMemcpyHostToDevice), "adapter upload");
+  });
+}
+
+int laya_b200_clear_adapter(laya_b200_engine* e, int slot) {
+  return guard(e, [&] {
+    if (!e->adapter_slots) fail("adapters are not enabled");
+    if (slot < 0 || slot >= e->adapter_slots) fail("adapter slot %d outside [0, %d)", slot, e->adapter_slots);
+    for (int i = 0; i < e->cfg.layers; ++i)
+      for (int w = 0; w < 4; ++w) {
+        const ParamInfo& pi = e->params.at("enc." + std::to_string(i) + "." + kAdapted[w]);
+        const AdapterSet& ad = e->adapters[i * 4 + w];
+        const size_t a = (size_t)e->adapter_rank * pi.cols, b = (size_t)e->adapter_rank * pi.rows;
+        ck(cudaMemset(ad.a + slot * a, 0, a * 2), "adapter clear");
+        ck(cudaMemset(ad.b + slot * b, 0, b * 2), "adapter clear");
+        ck(cudaMemset(ad.scaling + slot, 0, 4), "adapter clear");
+      }
+    ck(cudaDeviceSynchronize(), "adapter clear");
   });
 }
 
@@ -1335,16 +1564,19 @@ int laya_b200_finalize(laya_b200_engine* e, int precision) {
   });
 }
 
-int laya_b200_capture(laya_b200_engine* e, int batch, int seq, int options, int unmasked, int* slot) {
+namespace {
+
+int capture(laya_b200_engine* e, int batch, int seq, int options, int unmasked, int adapters, int* slot) {
   return guard(e, [&] {
     if (!e->finalized) fail("finalize the weights before capturing");
+    if (adapters && !e->adapter_slots) fail("adapters are not enabled");
     if (!slot) fail("null slot pointer");
     const laya_b200_config& c = e->cfg;
     if (batch < 1 || batch > c.max_batch) fail("batch %d outside [1, %d]", batch, c.max_batch);
     if (seq < 1 || seq > c.max_len) fail("seq %d outside [1, %d]", seq, c.max_len);
     if (options < 2 || options > c.max_options) fail("options %d outside [2, %d]", options, c.max_options);
     Slot s;
-    s.sh = Shape{batch, seq, options, unmasked ? 1 : 0};
+    s.sh = Shape{batch, seq, options, unmasked ? 1 : 0, adapters};
     try {
       s.io_exec = capture_graph(e, s.sh, kCatAll, true, &s.kernels);
       s.dev_exec[kCatAll] = capture_graph(e, s.sh, kCatAll, false, nullptr);
@@ -1365,6 +1597,16 @@ int laya_b200_capture(laya_b200_engine* e, int batch, int seq, int options, int 
   });
 }
 
+}  // namespace
+
+int laya_b200_capture(laya_b200_engine* e, int batch, int seq, int options, int unmasked, int* slot) {
+  return capture(e, batch, seq, options, unmasked, 0, slot);
+}
+
+int laya_b200_capture_adapters(laya_b200_engine* e, int batch, int seq, int options, int unmasked, int* slot) {
+  return capture(e, batch, seq, options, unmasked, 1, slot);
+}
+
 int laya_b200_release(laya_b200_engine* e, int slot) {
   return guard(e, [&] {
     if (slot < 0 || slot >= (int)e->slots.size() || !e->slots[slot].live) fail("no slot %d", slot);
@@ -1374,9 +1616,11 @@ int laya_b200_release(laya_b200_engine* e, int slot) {
   });
 }
 
-int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const int64_t* attention_mask,
-                  const int64_t* marker_pos, const uint8_t* marker_mask, const int64_t* qtype, float* logits,
-                  float* act) {
+namespace {
+
+int run(laya_b200_engine* e, int slot, const int64_t* input_ids, const int64_t* attention_mask,
+        const int64_t* marker_pos, const uint8_t* marker_mask, const int64_t* qtype, const int32_t* adapter,
+        float* logits, float* act) {
   return guard(e, [&] {
     if (slot < 0 || slot >= (int)e->slots.size() || !e->slots[slot].live) fail("no slot %d", slot);
     if (!input_ids || !attention_mask || !marker_pos || !marker_mask || !qtype || !logits || !act)
@@ -1385,6 +1629,7 @@ int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const
     const int b = sl.sh.b, s = sl.sh.s, k = sl.sh.k;
     const laya_b200_config& c = e->cfg;
     const IoLayout L = io_layout(sl.sh);
+    if (adapter && !sl.sh.adapters) fail("slot %d was captured without adapters", slot);
     int32_t* w = e->h_in;
     // Pack and validate on the host; nothing out of range reaches a kernel.
     for (int i = 0; i < b * s; ++i) {
@@ -1407,6 +1652,12 @@ int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const
         w[L.score + q * k + j] = q * (1 + k) + 1 + j;
       }
     }
+    if (sl.sh.adapters)
+      for (int q = 0; q < b; ++q) {
+        const int a = adapter ? adapter[q] : -1;
+        if (a < -1 || a >= e->adapter_slots) fail("adapter[%d]=%d outside [-1, %d)", q, a, e->adapter_slots);
+        w[L.adapter + q] = a;
+      }
     // The copy below overwrites the staging buffer with this slot's layout:
     // until it has completed, no slot's inputs are known to be resident.
     e->inputs_slot = -1;
@@ -1434,6 +1685,20 @@ int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const
     memcpy(logits, e->h_out + L.logits, sizeof(float) * b * k);
     memcpy(act, e->h_out + L.act, sizeof(float) * b * 2);
   });
+}
+
+}  // namespace
+
+int laya_b200_run(laya_b200_engine* e, int slot, const int64_t* input_ids, const int64_t* attention_mask,
+                  const int64_t* marker_pos, const uint8_t* marker_mask, const int64_t* qtype, float* logits,
+                  float* act) {
+  return run(e, slot, input_ids, attention_mask, marker_pos, marker_mask, qtype, nullptr, logits, act);
+}
+
+int laya_b200_run_adapters(laya_b200_engine* e, int slot, const int64_t* input_ids, const int64_t* attention_mask,
+                           const int64_t* marker_pos, const uint8_t* marker_mask, const int64_t* qtype,
+                           const int32_t* adapter, float* logits, float* act) {
+  return run(e, slot, input_ids, attention_mask, marker_pos, marker_mask, qtype, adapter, logits, act);
 }
 
 int laya_b200_replay_device(laya_b200_engine* e, int slot, int iterations, int kernel_mask, float* ms_each) {
@@ -1535,10 +1800,12 @@ int laya_b200_destroy(laya_b200_engine* e) {
       cudaFree(e->weights->qarena);
       cudaFree(e->weights->table_h);
       cudaFree(e->weights->table_qkv);
+      cudaFree(e->weights->adapters);
       delete e->weights;
     }
   }
   cudaFree(e->aarena);
+  cudaFree(e->lora_arena);
   cudaFree(e->d_in);
   cudaFree(e->d_out);
   if (e->h_in) cudaFreeHost(e->h_in);

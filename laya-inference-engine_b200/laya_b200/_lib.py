@@ -14,6 +14,8 @@ PRECISIONS = {"bf16": 0, "fp8": 1, "nvfp4": 2}
 
 EXPORTS = ("laya_b200_create", "laya_b200_set_weight", "laya_b200_finalize", "laya_b200_create_lane",
            "laya_b200_build_token_tables",
+           "laya_b200_enable_adapters", "laya_b200_set_adapter", "laya_b200_clear_adapter",
+           "laya_b200_capture_adapters", "laya_b200_run_adapters",
            "laya_b200_capture",
            "laya_b200_release", "laya_b200_run", "laya_b200_replay_device", "laya_b200_kernel_count",
            "laya_b200_read_buffer", "laya_b200_tail_noalloc", "laya_b200_test_withhold_stage",
@@ -84,6 +86,12 @@ def load():
         "laya_b200_create": (I, [I, ctypes.POINTER(Config), ctypes.POINTER(P)]),
         "laya_b200_create_lane": (I, [P, ctypes.POINTER(P)]),
         "laya_b200_build_token_tables": (I, [P]),
+        "laya_b200_enable_adapters": (I, [P, I, I]),
+        "laya_b200_set_adapter": (I, [P, I, ctypes.c_char_p, I, P, P, ctypes.c_float]),
+        "laya_b200_clear_adapter": (I, [P, I]),
+        "laya_b200_capture_adapters": (I, [P, I, I, I, I, ctypes.POINTER(I)]),
+        # as run, with the questions' adapter slots (int32) before the outputs
+        "laya_b200_run_adapters": (I, [P, I, P, P, P, P, P, P, P, P]),
         "laya_b200_set_weight": (I, [P, ctypes.c_char_p, P, ctypes.c_size_t]),
         "laya_b200_finalize": (I, [P, I]),
         "laya_b200_capture": (I, [P, I, I, I, I, ctypes.POINTER(I)]),

@@ -26,6 +26,7 @@ still stuck: its pool is shut down without waiting and its engine is left open
 (closing it under a running native call would free memory the call uses).
 """
 from concurrent.futures import ThreadPoolExecutor, wait as futures_wait
+from contextlib import contextmanager
 import threading
 
 import numpy as np
@@ -99,6 +100,9 @@ class B200Dispatcher:
         self.healthy = {d: True for d in self.devices}
         self.inflight = {d: None for d in self.devices}   # last future submitted to each worker
         self.lock = threading.Lock()
+        self.adapters = {}      # name -> (adapter, scaling), what every healthy GPU has loaded
+        self._gate = threading.Condition()
+        self._running, self._changing = 0, False    # run_items calls; a change of the adapters
         self.closed = False
 
     def _run_batches(self, device, items, batches):
@@ -119,6 +123,20 @@ class B200Dispatcher:
             raise RuntimeError("Dispatcher is closed")
         if not items:
             return []
+        with self._gate:
+            self._gate.wait_for(lambda: not self._changing)
+            unknown = {it["adapter"] for it in items if it.get("adapter") is not None} - set(self.adapters)
+            if unknown:  # the caller's error, not a GPU's
+                raise ValueError(f"no adapter {sorted(map(str, unknown))} is loaded")
+            self._running += 1
+        try:
+            return self._run_items(items)
+        finally:
+            with self._gate:
+                self._running -= 1
+                self._gate.notify_all()
+
+    def _run_items(self, items):
         results = {}
         pending = list(range(len(items)))
         errors = {}
@@ -159,6 +177,67 @@ class B200Dispatcher:
             pending = sorted(failed)
         return [results[i] for i in range(len(items))]
 
+    @contextmanager
+    def _changing_adapters(self):
+        """No run_items in progress; those that follow wait."""
+        with self._gate:
+            self._gate.wait_for(lambda: not self._changing)
+            self._changing = True
+            self._gate.wait_for(lambda: self._running == 0)
+        try:
+            yield
+        finally:
+            with self._gate:
+                self._changing = False
+                self._gate.notify_all()
+
+    def load_adapter(self, name, adapter, scaling=1.0):
+        """B200Engine.load_adapter on every healthy GPU, once no request is in
+        flight; items select it by their "adapter".  A GPU that is readmitted
+        later gets it then.  When a GPU refuses it, the others go back to what
+        they had and the error is raised."""
+        if self.closed:
+            raise RuntimeError("Dispatcher is closed")
+        # kept for readmitted GPUs, so not the caller's arrays
+        adapter = {k: tuple(np.array(x) for x in pair) for k, pair in adapter.items()}
+        with self._changing_adapters():
+            with self.lock:
+                alive = [d for d in self.devices if self.healthy[d]]
+            for i, d in enumerate(alive):
+                try:
+                    self.engines[d].load_adapter(name, adapter, scaling)
+                except Exception:
+                    for done in alive[:i + 1]:
+                        self._restore(done, name)
+                    raise
+            self.adapters[name] = (adapter, scaling)
+
+    def unload_adapter(self, name):
+        """B200Engine.unload_adapter on every healthy GPU, once no request is in flight."""
+        if self.closed:
+            raise RuntimeError("Dispatcher is closed")
+        with self._changing_adapters():
+            if name not in self.adapters:
+                raise ValueError(f"no adapter {name!r} is loaded")
+            del self.adapters[name]
+            with self.lock:
+                alive = [d for d in self.devices if self.healthy[d]]
+            for d in alive:
+                self._restore(d, name)
+
+    def _restore(self, device, name):
+        """Bring one adapter of one GPU to what self.adapters holds; a GPU that
+        cannot leaves service."""
+        engine = self.engines[device]
+        try:
+            if name in self.adapters:
+                engine.load_adapter(name, *self.adapters[name])
+            elif name in engine.adapters:
+                engine.unload_adapter(name)
+        except Exception:
+            with self.lock:
+                self.healthy[device] = False
+
     def _idle(self, device):
         fut = self.inflight[device]
         return fut is None or fut.done()
@@ -179,9 +258,18 @@ class B200Dispatcher:
             self.inflight[d] = fut
             futures_wait([fut], timeout=timeout if timeout is not None else self.timeout)
             if fut.done() and fut.exception() is None:
-                with self.lock:
-                    self.healthy[d] = True
-                back.append(d)
+                names = {*self.adapters, *getattr(self.engines[d], "adapters", ())}
+                if not names:
+                    with self.lock:
+                        self.healthy[d] = True
+                else:  # first what was loaded or unloaded while it was out
+                    with self._changing_adapters():
+                        with self.lock:
+                            self.healthy[d] = True
+                        for name in names:
+                            self._restore(d, name)
+                if self.healthy[d]:
+                    back.append(d)
         return back
 
     def close(self):

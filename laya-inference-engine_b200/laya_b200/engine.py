@@ -16,6 +16,7 @@ Mirrors ``src/laya_blackwell/engine.py``:
 The forward itself runs in liblaya_b200.so; there is no CPU path.
 """
 from collections import OrderedDict
+from contextlib import contextmanager
 import ctypes
 import queue
 import threading
@@ -26,7 +27,7 @@ import numpy as np
 from . import _lib
 from .config import LAYA, LayaConfig
 from .protocol import PreparedRequest, format_response, prepare_request
-from .weights import check_weights, seeded_weights, param_table
+from .weights import check_adapter, check_weights, seeded_weights, param_table
 from .workload import pack
 
 KEYS = ("input_ids", "attention_mask", "marker_pos", "marker_mask", "qtype")
@@ -79,10 +80,19 @@ class NativeForward:
         _lib.check(self.lib, self.handle, st, f"capture({batch},{seq},{options})")
         return slot.value
 
+    def capture_adapters(self, batch, seq, options, unmasked):
+        """capture() for batches whose questions select adapters."""
+        slot = ctypes.c_int()
+        st = self.lib.laya_b200_capture_adapters(self.handle, batch, seq, options, int(bool(unmasked)),
+                                                 ctypes.byref(slot))
+        _lib.check(self.lib, self.handle, st, f"capture_adapters({batch},{seq},{options})")
+        return slot.value
+
     def release(self, slot):
         _lib.check(self.lib, self.handle, self.lib.laya_b200_release(self.handle, slot), "release")
 
-    def run(self, slot, inputs):
+    def run(self, slot, inputs, adapter=None):
+        """`adapter` (slots of capture_adapters): adapter slot per question, -1 for none."""
         b, s = inputs["input_ids"].shape
         k = inputs["marker_pos"].shape[1]
         ids = np.ascontiguousarray(inputs["input_ids"], dtype=np.int64)
@@ -92,13 +102,38 @@ class NativeForward:
         qt = np.ascontiguousarray(inputs["qtype"], dtype=np.int64)
         logits = np.empty((b, k), dtype=np.float32)
         act = np.empty((b, 2), dtype=np.float32)
-        self.run_addresses(slot, tuple(a.ctypes.data for a in (ids, am, mp, mm, qt, logits, act)))
+        arrays = (ids, am, mp, mm, qt, logits, act)
+        if adapter is not None:
+            adapter = np.ascontiguousarray(adapter, dtype=np.int32)
+            if adapter.shape != (b,):
+                raise ValueError(f"adapter must name a slot for each of the {b} questions")
+            arrays = (*arrays[:5], adapter, *arrays[5:])
+        self.run_addresses(slot, tuple(a.ctypes.data for a in arrays))
         return logits, act
 
     def run_addresses(self, slot, addresses):
         """run() on host arrays given by address (ids, mask, marker_pos,
-        marker_mask, qtype, logits, act), for callers that keep them."""
-        _lib.check(self.lib, self.handle, self.lib.laya_b200_run(self.handle, slot, *addresses), "run")
+        marker_mask, qtype, [adapter,] logits, act), for callers that keep them."""
+        fn = self.lib.laya_b200_run if len(addresses) == 7 else self.lib.laya_b200_run_adapters
+        _lib.check(self.lib, self.handle, fn(self.handle, slot, *addresses), "run")
+
+    def enable_adapters(self, slots, max_rank):
+        """Reserve adapter slots (before lanes are created)."""
+        _lib.check(self.lib, self.handle, self.lib.laya_b200_enable_adapters(self.handle, slots, max_rank),
+                   "enable_adapters")
+
+    def set_adapter(self, slot, adapter, scaling=1.0):
+        """Replace the adapter in `slot` by ``{projection: (a, b)}`` (see
+        weights.check_adapter); no run may be in progress."""
+        adapter = check_adapter(adapter, self.cfg)
+        self.clear_adapter(slot)
+        for name, (a, b) in adapter.items():
+            st = self.lib.laya_b200_set_adapter(self.handle, slot, name.encode(), a.shape[0], a.ctypes.data,
+                                                b.ctypes.data, scaling)
+            _lib.check(self.lib, self.handle, st, f"set_adapter({name})")
+
+    def clear_adapter(self, slot):
+        _lib.check(self.lib, self.handle, self.lib.laya_b200_clear_adapter(self.handle, slot), "clear_adapter")
 
     def replay_device(self, slot, iterations, kernel_mask=15):
         """Per-replay device milliseconds of `iterations` back-to-back replays."""
@@ -169,11 +204,15 @@ class B200Engine:
     def __init__(self, model=None, *, weights=None, config: LayaConfig = LAYA, seed=0, device="cuda:0",
                  max_graphs=8, max_questions=64, sequence_buckets=(64, 128, 256, 384, 512, 768, 1024),
                  precision="bf16", max_options=256, tokenizer=None, agent_cfg=None, temperature=None,
-                 temperature_by_options=None, lanes=1, token_tables=False):
+                 temperature_by_options=None, lanes=1, token_tables=False, adapters=0, adapter_rank=16):
         if max_graphs < 1 or max_questions < 1:
             raise ValueError("max_graphs and max_questions must be positive")
         if lanes < 1:
             raise ValueError("lanes must be positive")
+        if adapters < 0 or not 1 <= adapter_rank <= 256:
+            raise ValueError("adapters must not be negative and adapter_rank be in [1, 256]")
+        if adapters and precision == "nvfp4":
+            raise ValueError("adapters run beside bf16 and fp8 weights, not nvfp4")
         if precision not in _lib.PRECISIONS:
             raise ValueError("precision must be bf16, fp8 or nvfp4")
         self.device = _device_index(device)
@@ -196,12 +235,17 @@ class B200Engine:
         self.native = NativeForward(self.device, config, weights, precision, max_batch=max_questions,
                                     max_options=max_options)
         self.max_options = max_options
-        if token_tables:  # before the lanes, which share them
-            try:
+        self.adapter_rank = adapter_rank
+        self.adapters = {}                             # name -> adapter slot
+        self._free_adapters = list(range(adapters))
+        try:  # before the lanes, which share both
+            if token_tables:
                 self.native.build_token_tables()
-            except Exception:
-                self.native.close()
-                raise
+            if adapters:
+                self.native.enable_adapters(adapters, adapter_rank)
+        except Exception:
+            self.native.close()
+            raise
         # Serving lanes: requests from concurrent callers run on idle lanes
         # (lane 0 is this object's own native / graphs); one lane serialises
         # every call like the reference's engine lock (engine.py:84,192).
@@ -246,6 +290,8 @@ class B200Engine:
         shape = self._shape(prepared)
         batch, length, _ = shape
         unmasked = len(prepared.items) == batch and all(len(item["ids"]) == length for item in prepared.items)
+        if any(item.get("adapter") is not None for item in prepared.items):
+            return (*shape, unmasked, "adapters")
         return (*shape, unmasked)
 
     def _fill(self, prepared, shape):
@@ -256,8 +302,10 @@ class B200Engine:
         """Pack into the slot's own host arrays (kept per graph key, addresses
         computed once) and run; same values as _fill + NativeForward.run."""
         lane = lane or self
+        adapted = len(key) > 4
         if not hasattr(lane.native, "run_addresses"):
-            return lane.native.run(slot, self._fill(prepared, key[:3]))
+            more = (self._adapter_slots(prepared, key[0]),) if adapted else ()
+            return lane.native.run(slot, self._fill(prepared, key[:3]), *more)
         io = getattr(lane, "_io", None)
         if io is None:
             io = lane._io = {}
@@ -274,6 +322,7 @@ class B200Engine:
                       "marker_pos": mpos.reshape(batch, options),
                       "marker_mask": np.empty((batch, options), np.uint8),
                       "qtype": qtype,
+                      **({"adapter": np.empty(batch, np.int32)} if adapted else {}),
                       "logits": np.empty((batch, options), np.float32),
                       "act": np.empty((batch, 2), np.float32)}
             clean_ints = np.zeros_like(ints)
@@ -295,8 +344,17 @@ class B200Engine:
             mpos[i, :k] = item["markers"]
             mmask[i, :k] = 1
             qtype[i] = item["qtype"]
+        if adapted:
+            arrays["adapter"][:] = self._adapter_slots(prepared, key[0])
         lane.native.run_addresses(slot, addresses)
         return arrays["logits"], arrays["act"]
+
+    def _adapter_slots(self, prepared, batch):
+        slots = np.full(batch, -1, np.int32)
+        for i, item in enumerate(prepared.items):
+            if item.get("adapter") is not None:
+                slots[i] = self.adapters[item["adapter"]]
+        return slots
 
     def _check_items(self, prepared, shape):
         _, length, options = shape
@@ -305,6 +363,9 @@ class B200Engine:
                 raise ValueError(f"question has {len(item['ids'])} tokens; the model maximum is {length}")
             if len(item["markers"]) > options or len(item["markers"]) > self.max_options:
                 raise ValueError(f"question has {len(item['markers'])} options; maximum is {self.max_options}")
+            name = item.get("adapter")
+            if name is not None and name not in getattr(self, "adapters", {}):
+                raise ValueError(f"no adapter {name!r} is loaded")
 
     def _slot(self, prepared, key=None, lane=None):
         lane = lane or self
@@ -317,7 +378,7 @@ class B200Engine:
             lane.native.release(old)
             getattr(lane, "_io", {}).pop(old_key, None)
         start = time.perf_counter()
-        slot = lane.native.capture(*key)
+        slot = lane.native.capture_adapters(*key[:4]) if len(key) > 4 else lane.native.capture(*key)
         lane.graphs[key] = slot
         return slot, True, (time.perf_counter() - start) * 1000
 
@@ -349,6 +410,53 @@ class B200Engine:
         return logits[:count].copy(), act[:count].copy(), {
             "graph_miss": miss, "graph_build_ms": build_ms if miss else 0.0, "shape": list(shape),
             "backend": self.backend, "precision": self.precision, "device": f"cuda:{self.device}"}
+
+    # -- adapters: per-question low-rank additions to the encoder projections
+    # (no counterpart in the reference).  An item's optional "adapter" names the
+    # one that its question runs with; a batch may mix them, and questions
+    # without one run on the shared weights alone.
+    def load_adapter(self, name, adapter, scaling=1.0):
+        """Load ``{projection: (a [r, in], b [out, r])}`` under `name` (see
+        weights.check_adapter; r at most adapter_rank), replacing one of that
+        name (lost if the upload fails).  Waits for the requests in flight."""
+        if name is None:
+            raise ValueError("an adapter needs a name")
+        adapter = check_adapter(adapter, self.config, self.adapter_rank)
+        if not np.isfinite(np.float32(scaling)):
+            raise ValueError("scaling must be finite")
+        with self._all_lanes():
+            if name not in self.adapters and not self._free_adapters:
+                raise RuntimeError("no adapter slot is free; unload one or create the engine with more adapters")
+            slot = self.adapters[name] if name in self.adapters else self._free_adapters.pop(0)
+            self.adapters.pop(name, None)  # not to be found half loaded
+            try:
+                self.native.set_adapter(slot, adapter, scaling)
+            except Exception:
+                self._free_adapters.append(slot)
+                raise
+            self.adapters[name] = slot
+
+    def unload_adapter(self, name):
+        """Free the slot of a loaded adapter.  Waits for the requests in flight."""
+        with self._all_lanes():
+            if name not in self.adapters:
+                raise ValueError(f"no adapter {name!r} is loaded")
+            slot = self.adapters.pop(name)
+            self._free_adapters.append(slot)
+            self.native.clear_adapter(slot)
+
+    @contextmanager
+    def _all_lanes(self):
+        """Every lane of this engine, idle and held."""
+        with self.lock:  # one caller at a time collects them
+            held = [self._idle.get() for _ in self._lanes]
+            try:
+                if self.closed:
+                    raise RuntimeError("Engine is closed")
+                yield
+            finally:
+                for lane in held:
+                    self._idle.put(lane)
 
     def predict(self, state, questions):
         start = time.perf_counter()

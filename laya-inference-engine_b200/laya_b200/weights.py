@@ -62,6 +62,46 @@ def param_table(cfg: LayaConfig = LAYA):
     return t
 
 
+def adapted_projections(cfg: LayaConfig = LAYA):
+    """Name -> (out_features, in_features) of the projections that an adapter
+    may extend: the encoder's, every layer's ``wqkv``, ``wo``, ``wi`` and ``wo2``."""
+    return {name: shape for name, shape, dtype, _ in param_table(cfg)
+            if name.startswith("enc.") and dtype == BF16}
+
+
+def check_adapter(adapter, cfg: LayaConfig = LAYA, max_rank=256):
+    """An adapter ``{projection: (a [r, in], b [out, r])}`` as bf16 bit patterns.
+
+    Arrays are bf16 bits (uint16) or floating point (rounded to bf16); ranks may
+    differ between projections.  Raises ValueError for an unknown projection, a
+    shape or rank that does not fit, or a value that is not finite."""
+    if not adapter:
+        raise ValueError("an adapter needs at least one projection")
+    known = adapted_projections(cfg)
+    out = {}
+    for name, pair in adapter.items():
+        if name not in known:
+            raise ValueError(f"no adapted projection {name!r}")
+        n, k = known[name]
+        bits = []
+        for x in pair:
+            x = np.asarray(x)
+            if x.dtype != np.uint16:
+                if not np.issubdtype(x.dtype, np.floating):
+                    raise ValueError(f"adapter {name!r}: arrays must be floating point or bf16 bits (uint16)")
+                x = f32_to_bf16_bits(x)
+            bits.append(np.ascontiguousarray(x))
+        a, b = bits
+        r = a.shape[0] if a.ndim == 2 else 0
+        if a.shape != (r, k) or b.shape != (n, r) or not 1 <= r <= max_rank:
+            raise ValueError(f"adapter {name!r}: a {a.shape} and b {b.shape} are not [r, {k}] and [{n}, r] with "
+                             f"1 <= r <= {max_rank}")
+        if not all(((x & 0x7F80) != 0x7F80).all() for x in bits):
+            raise ValueError(f"adapter {name!r} contains NaN or infinity")
+        out[name] = (a, b)
+    return out
+
+
 def f32_to_bf16_bits(x):
     """Round-to-nearest-even fp32 -> bf16, returned as uint16 bit patterns."""
     x = np.ascontiguousarray(x, dtype=np.float32)
