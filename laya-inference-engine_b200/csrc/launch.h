@@ -62,7 +62,9 @@ struct LoraMaps {
   CUtensorMap v;     // pairs: V as [rows][chunks * 64] bf16, 64 columns x 128 rows
   CUtensorMap out;   // pairs with p.tma_epilogue: output, 128 bytes of columns x 32 rows
 };
-cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl);
+// projection_ctas: CTAs of the projection behind it (launch_lora_pairs' grid), 0 for few rows.
+cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
+                               cudaStream_t stream, bool pdl);
 // Rows, and ranks of one adapter, in a CTA of the shrink.
 inline int lora_shrink_rows(int rows) { return rows <= 64 ? 64 : 128; }
 __host__ __device__ inline int lora_shrink_box(int rank) { return rank < 64 ? (rank + 15) / 16 * 16 : 64; }
@@ -74,6 +76,8 @@ void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split)
 // Without p.tma_epilogue (store epilogue only) the output may lie anywhere.
 cudaError_t launch_lora_pairs(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bnf,
                               cudaStream_t stream);
+// CTAs of launch_lora_pairs for these sizes (at most the SMs).
+int lora_pair_ctas(int M, int N, int bnf, int sm_count);
 // Features per tile of launch_lora_pairs, or 0 where launch_lora_gemm is to be used.
 int lora_pair_plan(int kind, int M, int N, int sm_count);
 // Status of the launches that were given no status word; reading clears it.

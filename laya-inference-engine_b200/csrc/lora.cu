@@ -65,19 +65,21 @@ constexpr int kShrinkPitch = kShrinkRanks + 4;
 constexpr int kShrinkXBytes = kShrinkRows * 128, kShrinkABytes = kShrinkCols * 128;
 constexpr int kShrinkPipe = kShrinkStages * (kShrinkXBytes + kShrinkABytes);
 static_assert(kShrinkRows * kShrinkPitch * 4 <= kShrinkPipe, "the partial sums lie over the stages");
-constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264) * 4 + 128 + 1024;
+constexpr int kListInts = 1536;  // write_list's memory
+constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264 + kListInts) * 4 + 128 + 1024;
 
 // The four warps that compute.
 DEVI void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Numbers the distinct non-negative values of own[] (row h * 128 + thread, 128
 // threads) in order of first appearance: ord[] of each row (-1: none), the
-// values in s_list, their count returned.  A warp's leaders look for their
+// values in s_list, their count returned (tid: 0..127).  A warp's leaders look for their
 // value among the earlier warps' leaders only, so a tile of long runs costs a
 // few steps.  s_tmp, s_entry: H * 128 ints (16-byte aligned); s_cnt: H * 4.
 template <int H>
-DEVI int number_adapters(const int (&own)[H], int (&ord)[H], int* s_list, int* s_tmp, int* s_entry, int* s_cnt) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_list, int* s_tmp, int* s_entry,
+                         int* s_cnt) {
+  const int lane = tid & 31, warp = tid >> 5;
   const unsigned below = (1u << lane) - 1;
   int lead[H], entry[H], seen[H];
   unsigned firsts[H];
@@ -134,7 +136,7 @@ DEVI void write_list(const LoraParams& p, int row0, int* w) {
   int own[2], ord[2] = {-1, -1};
   for (int h = 0; h < 2; ++h) own[h] = row_adapter(p, row0 + 128 * h + tid);
   int *s_list = w, *s_span = w + 256;
-  const int n = number_adapters<2>(own, ord, s_list, w + 768, w + 1024, w + 1280);
+  const int n = number_adapters<2>(tid, own, ord, s_list, w + 768, w + 1024, w + 1280);
   for (int j = tid; j < n; j += 128) {
     s_span[j] = 256;
     s_span[256 + j] = -1;
@@ -158,6 +160,61 @@ DEVI void write_list(const LoraParams& p, int row0, int* w) {
   if (tid == 0) out[0] = n;
 }
 
+// The sum of the K slices' parts of a row tile's kept columns, scaled, as V's
+// hi + lo pairs: sixteen lanes take a row (four ranks each), a thread four rows
+// at a time, whose parts are all requested before the first is added.
+// [t0, t1): the rows of this CTA; slot_of(row): the row's adapter, or -1 where
+// another pass or CTA holds it; r0: first rank of the columns.
+template <class SlotOf>
+DEVI void write_v(const LoraParams& p, const float* part, int row0, int t0, int t1, int cols, int r0, int split,
+                  SlotOf slot_of) {
+  const int c = (threadIdx.x & 15) * 4, r = r0 + c;
+  if (c >= cols || (r >> 5) >= p.chunks) return;
+  const uint32_t base = smem_u32(part);
+  for (int first = t0 + (int)(threadIdx.x >> 4); first < t1; first += 32) {
+    float4 sum[4];
+    int slot[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = first + 8 * i;
+      sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      slot[i] = row < t1 ? slot_of(row) : -1;
+    }
+    for (int k = 0; k < split; k += 2) {
+      float4 q[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (slot[i] >= 0 && k + j < split)
+            q[i][j] = ld_dsmem_f32x4(mapa_shared(base, k + j) + ((first + 8 * i) * kShrinkPitch + c) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (slot[i] >= 0 && k + j < split) {
+            sum[i].x += q[i][j].x;
+            sum[i].y += q[i][j].y;
+            sum[i].z += q[i][j].z;
+            sum[i].w += q[i][j].w;
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (slot[i] < 0) continue;
+      const float f = p.scaling ? p.scaling[slot[i]] : 1.f;
+      const float x[4] = {sum[i].x * f, sum[i].y * f, sum[i].z * f, sum[i].w * f};
+      float lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
+        lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
+      __nv_bfloat16* dst = p.v + ((size_t)(row0 + first + 8 * i) * p.chunks + (r >> 5)) * 64 + (r & 31);
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+      *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+    }
+  }
+}
+
 __global__ void __launch_bounds__(192)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
                        const LoraParams p) {
@@ -170,7 +227,7 @@ __global__ void __launch_bounds__(192)
   int* s_ord = reinterpret_cast<int*>(smem + kShrinkPipe);   // [128] each row's place in the list
   int* s_list = s_ord + 128;                                  // [128] distinct adapters
   int* s_tmp = s_list + 128;                                  // [128] + [128] + [4]: number_adapters
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264);
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264 + kListInts);
   uint64_t* empty = full + ST;
   uint64_t* done = empty + ST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -180,13 +237,6 @@ __global__ void __launch_bounds__(192)
   // projection launched behind it relies on that (its K blocks do not wait).
   griddep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
-  if ((int)blockIdx.x >= tiles) {  // the CTAs behind the row tiles write the projection's lists
-    griddep_launch_dependents();
-    if (blockIdx.y == 0 && blockIdx.z == 0 && warp < 4)
-      write_list(p, ((int)blockIdx.x - tiles) * 256, reinterpret_cast<int*>(smem));
-    return;
-  }
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, slices = gridDim.y / groups;
   const int group = blockIdx.y % groups, slice = blockIdx.y / groups;
   const int row0 = blockIdx.x * kShrinkRows, split = gridDim.z, rank = blockIdx.z;
@@ -218,7 +268,7 @@ __global__ void __launch_bounds__(192)
     // ---- the tile's adapters in order of first use (the rows are on their way)
     const int own[1] = {row_adapter(p, row0 + tid)};
     int ord[1] = {-1};
-    const int n = number_adapters<1>(own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
+    const int n = number_adapters<1>(tid, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
     s_ord[tid] = ord[0];
     if (tid == 0) *s_count = n;
   }
@@ -236,6 +286,8 @@ __global__ void __launch_bounds__(192)
       __syncwarp();
       if (!warp_wait(&full[k], 0, limit) && lane == 0) atomicExch(failed, 1);
     }
+  // the projection's list of 256 rows, while the first K blocks are on their way
+  if (warp < 4 && row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1) write_list(p, row0, s_tmp + 264);
   Ring<ST> ring;
   uint32_t g = 0, pass = 0;  // K blocks and passes before this one
   for (int u = u0; u < u1; u += per, ++pass) {
@@ -306,44 +358,12 @@ __global__ void __launch_bounds__(192)
     else
       __syncthreads();
     tc_fence_after();
-    if (warp < 4) {
-      const int t0 = rank * kShrinkRows / split, rows = (rank + 1) * kShrinkRows / split - t0;
-      const uint32_t base = smem_u32(part);
-      const int quads = cols / 4;
-      // four ranks of a row at a time; the parts of all K slices are requested
-      // before the first is added
-      for (int e = tid; e < rows * quads; e += 128) {
-        const int row = t0 + e / quads, c = e % quads * 4, r = group * kShrinkRanks + c, o = s_ord[row];
-        if (o < u || o >= u + units || (r >> 5) >= p.chunks) continue;
-        const int off = row * kShrinkPitch + c;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (split == 1) {
-          v = *reinterpret_cast<const float4*>(part + off);
-        } else {
-          float4 q[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < split) q[k] = ld_dsmem_f32x4(mapa_shared(base, k) + off * 4);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < split) {
-              v.x += q[k].x;
-              v.y += q[k].y;
-              v.z += q[k].z;
-              v.w += q[k].w;
-            }
-        }
-        const float f = p.scaling ? p.scaling[s_list[o]] : 1.f;
-        const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-        float lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
-          lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
-        __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-      }
-    }
+    if (warp < 4)
+      write_v(p, part, row0, rank * kShrinkRows / split, (rank + 1) * kShrinkRows / split, cols, group * kShrinkRanks,
+              split, [&](int row) {
+                const int o = s_ord[row];
+                return o >= u && o < u + units ? s_list[o] : -1;
+              });
     // the partial sums are read; the next pass's copies may take their place
     fence_proxy_async_smem();
     if (split > 1)
@@ -418,10 +438,6 @@ __global__ void __launch_bounds__(160)
   const bool loader = warp == 4;
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, slices = gridDim.y / groups;
   const int group = blockIdx.y % groups, slice = blockIdx.y / groups;
-  if (blockIdx.x == 1) {  // these CTAs write the projection's list
-    if (blockIdx.y == 0 && blockIdx.z == 0 && !loader) write_list(p, 0, reinterpret_cast<int*>(smem));
-    return;
-  }
   const int split = gridDim.z, rank = blockIdx.z;
   const int cols = lora_shrink_box(p.rank);  // of one adapter
   const int kblocks = (p.in_features + 63) / 64;
@@ -447,7 +463,7 @@ __global__ void __launch_bounds__(160)
     // ---- the tile's adapters in order of first use (the rows are on their way)
     const int own[1] = {tid < kFewRows ? row_adapter(p, tid) : -1};
     int ord[1] = {-1};
-    const int n = number_adapters<1>(own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
+    const int n = number_adapters<1>(tid, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
     s_ord[tid] = ord[0];
     if (tid == 0) *s_count = n;
   }
@@ -528,44 +544,12 @@ __global__ void __launch_bounds__(160)
       cluster_sync_all();
     else
       __syncthreads();
-    if (!loader) {
-      const int t0 = rank * kFewRows / split, rows = (rank + 1) * kFewRows / split - t0;
-      const uint32_t base = smem_u32(part);
-      const int quads = cols / 4;
-      // four ranks of a row at a time; the parts of all K slices are requested
-      // before the first is added
-      for (int e = tid; e < rows * quads; e += 128) {
-        const int row = t0 + e / quads, c = e % quads * 4, r = group * kShrinkRanks + c, o = s_ord[row];
-        if (o < u || o >= u + units || (r >> 5) >= p.chunks) continue;
-        const int off = row * kShrinkPitch + c;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (split == 1) {
-          v = *reinterpret_cast<const float4*>(part + off);
-        } else {
-          float4 q[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < split) q[k] = ld_dsmem_f32x4(mapa_shared(base, k) + off * 4);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < split) {
-              v.x += q[k].x;
-              v.y += q[k].y;
-              v.z += q[k].z;
-              v.w += q[k].w;
-            }
-        }
-        const float f = p.scaling ? p.scaling[s_list[o]] : 1.f;
-        const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-        float lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
-          lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
-        __nv_bfloat16* dst = p.v + ((size_t)row * p.chunks + (r >> 5)) * 64 + (r & 31);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-      }
-    }
+    if (!loader)
+      write_v(p, part, 0, rank * kFewRows / split, (rank + 1) * kFewRows / split, cols, group * kShrinkRanks, split,
+              [&](int row) {
+                const int o = s_ord[row];
+                return o >= u && o < u + units ? s_list[o] : -1;
+              });
     // the partial sums are read; the next pass's copies may take their place
     fence_proxy_async_smem();
     if (split > 1)
@@ -584,7 +568,8 @@ __global__ void __launch_bounds__(160)
 // last row, so 64 single rows with 64 adapters cost as many narrow MMAs; four
 // builder warps prepare the V tiles, each its own blocks, loading the next
 // one's values before they wait for its stage.
-constexpr int kFewBuilders = 4;  // warps; divides STAGES (each sees every use of its stages)
+constexpr int kFewBuilders = 4;  // warps, two for each of two stages in turn; half of them divides STAGES, so that
+                                 // each sees every use of its stages
 
 template <int BN, int KIND>
 struct LoraCfg {
@@ -596,7 +581,7 @@ struct LoraCfg {
   static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
   static constexpr int PART_BYTES = BN * 128 * 4;
   static constexpr int MAIN_BYTES = PIPE_BYTES > PART_BYTES ? PIPE_BYTES : PART_BYTES;
-  static constexpr int LIST_BYTES = BN * 12;  // distinct adapters, their rows, activation scales
+  static constexpr int LIST_BYTES = (128 + 2 * BN + 264) * 4;  // adapters, their rows, numbering, activation scales
   static constexpr int BAR_BYTES = 256;
   static constexpr int SMEM = MAIN_BYTES + BAR_BYTES + LIST_BYTES + 1024;
   static constexpr int ACCS = KIND == kKindFp8 ? 2 : 1;
@@ -631,7 +616,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
                      const __grid_constant__ CUtensorMap bmap, const GemmParams p, const LoraParams lp) {
   using C = LoraCfg<BN, KIND>;
   constexpr int STAGES = C::STAGES;
-  static_assert(STAGES % kFewBuilders == 0, "builder warps and stages");
+  static_assert(STAGES % (kFewBuilders / 2) == 0 && kFewBuilders == 4, "builder warps and stages");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -644,11 +629,12 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   uint64_t* listed = done + 1;  // the tile's adapter list is in shared memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(listed + 1);
   uint32_t* failed = tmem_slot + 1;
-  int* s_count = reinterpret_cast<int*>(failed + 1);
-  static_assert((4 * STAGES + 2) * 8 + 12 <= C::BAR_BYTES, "barrier block");
-  int* s_list = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [BN] distinct adapters
-  int* s_span = s_list + BN;                                                  // [BN] first | last << 16 of their rows
-  float* s_scale = reinterpret_cast<float*>(s_span + BN);                     // [BN] activation scales (fp8)
+  int* s_count = reinterpret_cast<int*>(failed + 1);  // distinct adapters, widest span of rows
+  static_assert((4 * STAGES + 2) * 8 + 16 <= C::BAR_BYTES, "barrier block");
+  int* s_list = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [128] distinct adapters
+  int* s_span = s_list + 128;                                                 // [BN] first | last << 16 of their rows
+  int* s_tmp = s_span + BN;                                                   // [264] number_adapters
+  float* s_scale = reinterpret_cast<float*>(s_tmp + 264);                     // [BN] activation scales (fp8)
 
   const int tid = threadIdx.x, warp = tid >> 5;
   const int tile_n = blockIdx.x;
@@ -662,7 +648,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&vfull[s], 1);
+      mbar_init(&vfull[s], 2);  // the stage's two halves
       mbar_init(&vfree[s], 1);
     }
     mbar_init(done, 1);
@@ -686,12 +672,18 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
 
   const uint64_t limit = wait_limit(p.wait_limit_us);
   int issued = 0;  // producer warp: loads issued (for the drain on failure)
-  // This rank's share [b0, b1) of the tile's adapter blocks (adapter, chunk of
-  // 32 ranks); known once `listed` has completed.
-  auto blocks = [&](int& b0, int& b1) {
+  // This rank's share of the tile's adapter blocks (adapter, chunk of 32
+  // ranks), known once `listed` has completed: [b0, b1), `pack` of them in a
+  // stage.  A stage has room for two blocks of half the rows each, which single
+  // rows' adapters are; two at a time keep twice the loads in flight.
+  struct Share {
+    int b0, b1, pack;
+    DEVI int stages() const { return (b1 - b0 + pack - 1) / pack; }
+  };
+  auto share = [&] {
     const int n = s_count[0] * lp.chunks;
-    b0 = (int)((long long)rank * n / split);
-    b1 = (int)((long long)(rank + 1) * n / split);
+    return Share{(int)((long long)rank * n / split), (int)((long long)(rank + 1) * n / split),
+                 s_count[1] <= BN / 2 && KIND == kKindBf16 ? 2 : 1};
   };
   // Rows [c0, c1) that block b multiplies: whole groups of 16.  The first block
   // of the FP8 kernels takes every row, which starts their second accumulator.
@@ -724,39 +716,33 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     }
     ok = ok && warp_wait(listed, 0, limit);
     if (ok) {
-      int b0, b1;
-      blocks(b0, b1);
-      for (int b = b0; b < b1; ++b, ring.next()) {
-        const int i = nkb + b - b0, s = ring.s;
+      const Share sh = share();
+      for (int q = 0; q < sh.stages(); ++q, ring.next()) {
+        const int i = nkb + q, s = ring.s, b = sh.b0 + q * sh.pack, two = sh.pack == 2 && b + 1 < sh.b1;
         if (i >= STAGES && !(ok = warp_wait(&empty[s], ring.phase ^ 1, limit))) break;
         if (elect_one()) {
           mbar_arrive(&vfree[s]);
-          mbar_expect_tx(&full[s], 128 * 64);
-          tma_load_3d(sA + s * C::A_BYTES, &bmap, &full[s], (b % lp.chunks) * 32, tile_n * 128, s_list[b / lp.chunks],
-                      pol_w);
+          mbar_expect_tx(&full[s], two ? 2 * 128 * 64 : 128 * 64);
+          for (int h = 0; h <= two; ++h)
+            tma_load_3d(sA + s * C::A_BYTES + h * 128 * 64, &bmap, &full[s], ((b + h) % lp.chunks) * 32, tile_n * 128,
+                        s_list[(b + h) / lp.chunks], pol_w);
         }
         __syncwarp();
         issued = i + 1;
       }
+      // every stage's last release, so that none is in flight at the exit
+      for (int i = issued < STAGES ? 0 : issued - STAGES; ok && i < issued; ++i)
+        ok = warp_wait(&empty[i % STAGES], (i / STAGES) & 1, limit);
     }
     if (!ok && (tid & 31) == 0) give_up(kStatusGemmEmptyTimeout);
   } else if (warp == 1) {
     const uint32_t idesc = KIND == kKindBf16 ? idesc_bf16(128, BN) : idesc_e4m3(128, BN);
     const uint32_t a0 = desc_lo(smem_u32(sA)), d0 = desc_lo(smem_u32(sB));
     Ring<STAGES> ring;
-    bool ok = true, known = false;
-    int b0 = 0, b1 = 0, total = nkb;
+    bool ok = true;
     for (int i = 0; i < nkb; ++i, ring.next()) {
       const int s = ring.s;
       if (!(ok = warp_wait(&full[s], ring.phase, limit))) break;
-      // Only stages that are refilled get a release (nothing is left in
-      // flight when the CTA exits); near the end that takes the block count.
-      if (i + STAGES >= nkb && !known) {
-        if (!(ok = warp_wait(listed, 0, limit))) break;
-        blocks(b0, b1);
-        total = nkb + b1 - b0;
-        known = true;
-      }
       tc_fence_after();
       if (elect_one()) {
         const uint32_t ad = a0 + s * (C::A_BYTES >> 4), bd = d0 + s * (C::B_BYTES >> 4);
@@ -767,78 +753,109 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
           else
             umma1_f8(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
         }
-        if (i + STAGES < total) umma_commit(&empty[s]);
+        umma_commit(&empty[s]);
       }
       __syncwarp();
     }
-    for (int b = b0; b < b1 && ok; ++b, ring.next()) {
-      const int i = nkb + b - b0, s = ring.s;
-      if (!(ok = warp_wait(&full[s], ring.phase, limit)) ||
-          !(ok = warp_wait(&vfull[s], ((b - b0) / STAGES) & 1, limit)))
-        break;
-      tc_fence_after();
-      int c0, c1;
-      span(b, b0, c0, c1);
-      if (elect_one()) {
-        const uint32_t ad = a0 + s * (C::A_BYTES >> 4), bd = d0 + s * (C::B_BYTES >> 4);
-        const uint32_t id2 = idesc_bf16(128, c1 - c0), acc = tmem2 + c0;
-        umma1_f16<kDesc64, kDesc128>(acc, ad, bd, id2, KIND == kKindBf16 || b > b0);  // hi
-        umma1_f16<kDesc64, kDesc128>(acc, ad, bd + 4, id2, 1);                        // lo
-        if (lp.rank - (b % lp.chunks) * 32 > 16) {
-          umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 2, id2, 1);
-          umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 6, id2, 1);
+    if (ok && (ok = warp_wait(listed, 0, limit))) {
+      const Share sh = share();
+      for (int q = 0; q < sh.stages(); ++q, ring.next()) {
+        const int s = ring.s, b = sh.b0 + q * sh.pack, two = sh.pack == 2 && b + 1 < sh.b1;
+        if (!(ok = warp_wait(&full[s], ring.phase, limit)) || !(ok = warp_wait(&vfull[s], (q / STAGES) & 1, limit)))
+          break;
+        tc_fence_after();
+        if (elect_one()) {
+          for (int h = 0; h <= two; ++h) {
+            int c0, c1;
+            span(b + h, sh.b0, c0, c1);
+            const uint32_t ad = a0 + s * (C::A_BYTES >> 4) + h * (128 * 64 >> 4);
+            const uint32_t bd = d0 + s * (C::B_BYTES >> 4) + h * (C::B_BYTES / 2 >> 4);
+            const uint32_t id2 = idesc_bf16(128, c1 - c0), acc = tmem2 + c0;
+            umma1_f16<kDesc64, kDesc128>(acc, ad, bd, id2, KIND == kKindBf16 || b > sh.b0);  // hi
+            umma1_f16<kDesc64, kDesc128>(acc, ad, bd + 4, id2, 1);                           // lo
+            if (lp.rank - ((b + h) % lp.chunks) * 32 > 16) {
+              umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 2, id2, 1);
+              umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 6, id2, 1);
+            }
+          }
+          umma_commit(&empty[s]);
         }
-        if (i + STAGES < total) umma_commit(&empty[s]);
+        __syncwarp();
       }
-      __syncwarp();
     }
     if (!ok && (tid & 31) == 0) give_up(kStatusGemmFullTimeout);
     if (elect_one()) umma_commit(done);
     __syncwarp();
   } else if (warp >= 2) {
-    // ---- the list, then the V tiles: rows of other adapters are zero
-    constexpr int BUILDERS = 32 * kFewBuilders;
+    // ---- the tile's adapters in order of first use and the rows each spans
+    // (which do not wait for the shrink), then the V tiles: rows of other
+    // adapters are zero
     const int bt = tid - 64, lane = tid & 31, bw = bt >> 5;
-    const int own0 = row_adapter(lp, lane), own1 = BN > 32 ? row_adapter(lp, lane + 32) : -1;
-    griddep_wait();  // the list and V
-    const int n = min(lp.lists[0], BN);
+    const int own[1] = {bt < BN ? row_adapter(lp, bt) : -1};
+    int ord[1] = {-1};
+    const int n = number_adapters<1>(bt, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
+    int *s_first = s_tmp, *s_last = s_tmp + 128;
+    sync128();
     if (bt < n) {
-      s_list[bt] = lp.lists[kLoraListSlots + bt];
-      s_span[bt] = lp.lists[kLoraListSpans + bt];
+      s_first[bt] = BN;
+      s_last[bt] = -1;
     }
-    if (bt == 0) s_count[0] = n;
-    asm volatile("bar.sync 1, %0;" ::"n"(BUILDERS) : "memory");
+    if (bt == 0) {
+      s_count[0] = n;
+      s_count[1] = 0;
+    }
+    sync128();
+    const unsigned same = __match_any_sync(0xffffffffu, ord[0]);
+    if (ord[0] >= 0 && __ffs(same) - 1 == lane) {  // one lane of a warp's run speaks for it
+      atomicMin(&s_first[ord[0]], bt);
+      atomicMax(&s_last[ord[0]], bt - lane + 31 - __clz(same));
+    }
+    sync128();
+    if (bt < n) {
+      s_span[bt] = s_first[bt] | s_last[bt] << 16;
+      atomicMax(&s_count[1], ((s_last[bt] + 16) & ~15) - (s_first[bt] & ~15));
+    }
+    sync128();
     if (bt == 0) mbar_arrive(listed);
-    int b0, b1;
-    blocks(b0, b1);
-    const int j = lane & 7;  // 16-byte chunk of a V row
-    for (int b = b0 + bw; b < b1; b += kFewBuilders) {
-      const int s = (nkb + b - b0) % STAGES, c = b % lp.chunks, slot = s_list[b / lp.chunks];
-      const int ksteps = lp.rank - c * 32 > 16 ? 2 : 1;
-      int c0, c1;
-      span(b, b0, c0, c1);
+    const Share sh = share();
+    const int half = bw & 1, j = lane & 7;  // half of a stage; 16-byte chunk of a V row
+    const int own0 = row_adapter(lp, lane), own1 = BN > 32 ? row_adapter(lp, lane + 32) : -1;
+    griddep_wait();  // V
+    // a warp takes its half of every second stage and loads the next block's
+    // values before it waits for the stage
+    for (int q = bw >> 1; q < sh.stages(); q += kFewBuilders / 2) {
+      const int s = (nkb + q) % STAGES, b = sh.b0 + q * sh.pack + half;
+      const bool has = half < sh.pack && b < sh.b1;
       uint4 v[BN / 4];
+      int c0 = 0, c1 = 0;
+      if (has) {
+        const int c = b % lp.chunks, slot = s_list[b / lp.chunks];
+        const int ksteps = lp.rank - c * 32 > 16 ? 2 : 1;
+        span(b, sh.b0, c0, c1);
 #pragma unroll
-      for (int u = 0; u < BN / 4; ++u) {
-        const int row = c0 + u * 4 + (lane >> 3);
-        const int o0 = __shfl_sync(0xffffffffu, own0, row & 31), o1 = __shfl_sync(0xffffffffu, own1, row & 31);
-        v[u] = make_uint4(0, 0, 0, 0);
-        if (row < c1 && (row < 32 ? o0 : o1) == slot && (j & 3) < 2 * ksteps)
-          v[u] = *reinterpret_cast<const uint4*>(lp.v + ((size_t)row * lp.chunks + c) * 64 + j * 8);
+        for (int u = 0; u < BN / 4; ++u) {
+          const int row = c0 + u * 4 + (lane >> 3);
+          const int o0 = __shfl_sync(0xffffffffu, own0, row & 31), o1 = __shfl_sync(0xffffffffu, own1, row & 31);
+          v[u] = make_uint4(0, 0, 0, 0);
+          if (row < c1 && (row < 32 ? o0 : o1) == slot && (j & 3) < 2 * ksteps)
+            v[u] = *reinterpret_cast<const uint4*>(lp.v + ((size_t)row * lp.chunks + c) * 64 + j * 8);
+        }
       }
       // (the builders cannot wait on `empty` themselves: they have not followed
       // its phases through the K blocks, and a parity names every second one)
-      if (!warp_wait(&vfree[s], ((b - b0) / STAGES) & 1, limit)) {
+      if (!warp_wait(&vfree[s], (q / STAGES) & 1, limit)) {
         if (lane == 0) give_up(kStatusGemmEmptyTimeout);
         break;
       }
-      uint8_t* dst = sB + s * C::B_BYTES;
+      if (has) {
+        uint8_t* dst = sB + s * C::B_BYTES + half * (C::B_BYTES / 2);
 #pragma unroll
-      for (int u = 0; u < BN / 4; ++u) {
-        const int row = u * 4 + (lane >> 3);
-        if (c0 + row < c1) *reinterpret_cast<uint4*>(dst + sw128_offset(row, j)) = v[u];
+        for (int u = 0; u < BN / 4; ++u) {
+          const int row = u * 4 + (lane >> 3);
+          if (c0 + row < c1) *reinterpret_cast<uint4*>(dst + sw128_offset(row, j)) = v[u];
+        }
+        fence_proxy_async_smem();
       }
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[s]);
     }
@@ -852,13 +869,10 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   if (!warp_wait(done, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
   tc_fence_after();
   __syncthreads();
-  const bool gpath = split > 1 && p.partials != nullptr;
   float* part = reinterpret_cast<float*>(smem);
-  if (gpath) part = p.partials + ((size_t)tile_n * split + rank) * BN * 128;
   {
-    int b0, b1;
-    blocks(b0, b1);
-    const bool second = KIND == kKindFp8 && b1 > b0;
+    const Share sh = share();
+    const bool second = KIND == kKindFp8 && sh.b1 > sh.b0;
     const int lq = warp & 3;
     const int lr = lq * 32 + (tid & 31);  // weight row of the tile
     const uint32_t lane_addr = (uint32_t)(lq * 32) << 16;
@@ -915,15 +929,9 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           if (u < split) {
-            if (gpath) {
-              const float* src = p.partials + ((size_t)tile_n * split + u) * BN * 128 + off;
-              va[u] = __ldcg(reinterpret_cast<const float4*>(src));
-              vb[u] = __ldcg(reinterpret_cast<const float4*>(src + pair));
-            } else {
-              const uint32_t base = mapa_shared(part_addr, (uint32_t)u);
-              va[u] = ld_dsmem_f32x4(base + off * 4);
-              vb[u] = ld_dsmem_f32x4(base + (off + pair) * 4);
-            }
+            const uint32_t base = mapa_shared(part_addr, (uint32_t)u);
+            va[u] = ld_dsmem_f32x4(base + off * 4);
+            vb[u] = ld_dsmem_f32x4(base + (off + pair) * 4);
           }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
@@ -942,7 +950,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       }
     }
   }
-  if (split > 1 && !gpath) cluster_sync_all();
+  if (split > 1) cluster_sync_all();
 
   // ---- teardown: drain copies still in flight after a failure, free TMEM
   if (tid == 0 && *failed) {
@@ -1035,7 +1043,8 @@ cudaError_t launch_shrink(const void* kern, int smem, int threads, dim3 grid, co
 
 }  // namespace
 
-cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, cudaStream_t stream, bool pdl) {
+cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
+                               cudaStream_t stream, bool pdl) {
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
       p.index_div < 1 || !p.lists)
     return cudaErrorInvalidValue;
@@ -1064,19 +1073,22 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
     const int slices = std::min(room, (std::min(p.slots, p.rows) + per - 1) / per);
     int split = 1;
     while (split < 8 && 2 * split <= kblocks && 2 * split * slices <= room) split *= 2;
-    const dim3 grid(2, groups * slices, split);
+    const dim3 grid(1, groups * slices, split);
     return wide ? launch_shrink((const void*)lora_shrink_few_kernel<true>, kWide, 160, grid, maps, p, stream, pdl)
                 : launch_shrink((const void*)lora_shrink_few_kernel<false>, kSlim, 160, grid, maps, p, stream, pdl);
   }
   // One CTA per SM: K is split until they are in use (two K blocks at least
   // each), then the adapters, of which single rows of many requests bring many.
   const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
-  const int room = std::max(1, sm_count / (tiles * groups));
+  // (the SMs that the projection's CTAs leave, where it does not need them all:
+  // both then run side by side)
+  const int free_sms = sm_count - projection_ctas;
+  const int room = std::max(1, (free_sms >= tiles * groups ? free_sms : sm_count) / (tiles * groups));
   int split = 1;
   while (split < 8 && 4 * split <= kblocks && 2 * split <= room) split *= 2;
   const int slices = std::max(1, std::min(room / split, std::min(p.slots, std::min(p.rows, kShrinkRows))));
   return launch_shrink((const void*)lora_shrink_kernel, kShrinkSmem, 192,
-                       dim3(tiles + (p.rows + 255) / 256, groups * slices, split), maps, p, stream, pdl);
+                       dim3(tiles, groups * slices, split), maps, p, stream, pdl);
 }
 
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,

@@ -122,16 +122,24 @@ DEVI void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::
 // columns n.. where the output's rows do not take TMA stores (unaligned rows or
 // strides): its lanes store along the rows.
 DEVI void store_block(const GemmParams& p, int m0, int n, const uint8_t* block) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int r = 0; r < 32; ++r) {
-    if (m0 + r >= p.M) break;
-    __nv_bfloat16* dst = p.out + (size_t)(m0 + r) * p.ldo + n;
+  const int lane = threadIdx.x & 31, rows = min(32, p.M - m0);
+  const bool in0 = n + lane < p.N, in1 = n + lane + 32 < p.N;
+  const uint8_t* src = block + (lane & 7) * 2;
+  const int c0 = lane >> 3, c1 = c0 + 4;
+  __nv_bfloat16* dst = p.out + (size_t)m0 * p.ldo + n + lane;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = lane + 32 * h;
-      if (n + c < p.N)
-        dst[c] = *reinterpret_cast<const __nv_bfloat16*>(block + sw128_offset(r, c >> 3) + (c & 7) * 2);
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    __nv_bfloat16 a[8], b[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      a[r] = *reinterpret_cast<const __nv_bfloat16*>(src + sw128_offset(r0 + r, c0));
+      b[r] = *reinterpret_cast<const __nv_bfloat16*>(src + sw128_offset(r0 + r, c1));
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      __nv_bfloat16* row = dst + (size_t)(r0 + r) * p.ldo;
+      if (r0 + r < rows && in0) row[0] = a[r];
+      if (r0 + r < rows && in1) row[32] = b[r];
     }
   }
 }
@@ -589,6 +597,11 @@ int lora_pair_plan(int kind, int M, int N, int sm_count) {
   const long long wide = (tm * ((N + 255) / 256) + pairs - 1) / pairs;
   const long long slim = (tm * ((N + 127) / 128) + pairs - 1) / pairs;
   return 10 * wide <= 7 * slim ? 256 : 128;
+}
+
+int lora_pair_ctas(int M, int N, int bnf, int sm_count) {
+  const long long tiles = (long long)((M + 255) / 256) * ((N + bnf - 1) / bnf);
+  return (int)std::min<long long>(2 * tiles, sm_count);
 }
 
 cudaError_t launch_lora_pairs(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bnf,

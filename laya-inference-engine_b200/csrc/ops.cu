@@ -56,8 +56,8 @@ struct LoraPlan {
   int kind, kblocks;
   int bnf;        // features per tile of the pair kernel, or 0:
   int bn, split;  // row tile and K split of the kernel for few rows
-  size_t v_bytes, list_bytes, partial_bytes;
-  size_t bytes() const { return v_bytes + list_bytes + partial_bytes; }
+  size_t v_bytes, list_bytes;
+  size_t bytes() const { return v_bytes + list_bytes; }
 };
 
 constexpr int kMaxRows = 1 << 22, kMaxFeatures = 1 << 20;
@@ -83,13 +83,8 @@ bool lora_plan(const laya_b200_lora_args* a, int sm_count, LoraPlan* plan) {
   auto align_up = [](size_t x) { return (x + 255) / 256 * 256; };
   plan->v_bytes = align_up((size_t)rows * ((a->rank + 31) / 32) * 128);
   plan->list_bytes = align_up((size_t)((rows + 255) / 256) * kLoraListInts * sizeof(int));
-  plan->partial_bytes = 0;
   plan->bnf = lora_pair_plan(plan->kind, rows, a->out_features, sm_count);
-  if (!plan->bnf) {
-    lora_few_plan(rows, a->out_features, plan->kblocks, sm_count, &plan->bn, &plan->split);
-    if (plan->split > 1)
-      plan->partial_bytes = (size_t)((a->out_features + 127) / 128) * plan->split * plan->bn * 128 * sizeof(float);
-  }
+  if (!plan->bnf) lora_few_plan(rows, a->out_features, plan->kblocks, sm_count, &plan->bn, &plan->split);
   return true;
 }
 
@@ -223,9 +218,9 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     p.a_scale = a->code_scale;
     p.w_scale = a->weight_scale;
     lp.lists = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
-    if (plan.partial_bytes) p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t err = launch_lora_shrink(maps, lp, sms, st, true);
+    cudaError_t err = launch_lora_shrink(
+        maps, lp, sms, plan.bnf ? lora_pair_ctas(M, N, plan.bnf, sms) : 0, st, true);
     if (err != cudaSuccess) return reject("adapter shrink launch", err);
     err = plan.bnf ? launch_lora_pairs(plan.kind, maps, p, lp, plan.bnf, st)
                    : launch_lora_gemm(plan.kind, maps, p, lp, plan.bn, plan.split, st);
