@@ -35,9 +35,10 @@ struct PairCfg {
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BNF / 2 * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 128 * 1024 / STAGE_BYTES;  // more measured no faster, and the shrink shares the SM
+  // Loads take up to 1.7 us while every SM stores: six stages of 32 KB hide it.
+  static constexpr int STAGES = 192 * 1024 / STAGE_BYTES;
   static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int STAGING_BYTES = 4 * 2 * 32 * 128;  // per epilogue warp two blocks of 32 rows x 128 bytes
+  static constexpr int STAGING_BYTES = 4 * 32 * 128;  // per epilogue warp a block of 32 rows x 128 bytes
   static constexpr int COLS_BYTES = 2 * BNF * 4;     // per column: weight scale, bias
   static constexpr int BAR_BYTES = 512;
   static constexpr int SMEM = PIPE_BYTES + STAGING_BYTES + BAR_BYTES + COLS_BYTES + 1024;
@@ -116,7 +117,6 @@ DEVI void tma_add_2d(const CUtensorMap* map, const void* src, int x, int y) {
                "r"(smem_u32(src)), "r"(x), "r"(y)
                : "memory");
 }
-DEVI void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 
 // A warp's block of 32 rows x 64 bf16 columns (128-byte swizzle) to rows m0..,
 // columns n.. where the output's rows do not take TMA stores (unaligned rows or
@@ -401,8 +401,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     // at a time go through a swizzled block to a TMA store of the warp's 32 rows
     griddep_wait();
     const int lq = warp - 4;
-    uint8_t* stage = staging + lq * 2 * 32 * 128;
-    uint32_t n = 0, block = 0;
+    uint8_t* dst = staging + lq * 32 * 128;
+    uint32_t n = 0;
     for (int t = pair; t < tiles; t += pairs, ++n) {
       const int tm = t % tiles_m, tn = t / tiles_m, buf = n & 1;
       const int mw = tm * 256 + (int)rank * 128 + lq * 32, m = mw + lane, n0 = tn * BNF;
@@ -460,17 +460,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       };
       constexpr int STEP = EPI == kPairGeglu ? 128 : EPI == kPairResidual ? 32 : 64;
 #pragma unroll 1
-      for (int c = 0; c < BNF && n0 + c < p.N; c += STEP, ++block) {
-        uint8_t* dst = stage + (block & 1) * 32 * 128;
-        // the store that read this block two steps ago has finished with it
-        if (lane == 0) bulk_wait_read1();
-        __syncwarp();
+      for (int c = 0; c < BNF && n0 + c < p.N; c += STEP) {
         auto put = [&](int j, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
           *reinterpret_cast<uint4*>(dst + sw128_offset(lane, j)) = make_uint4(a, b, d, e);
+        };
+        // the last store has finished reading the block by the time the sums are
+        // here; nothing is written to it before
+        auto block_free = [&] {
+          if (lane == 0) bulk_wait_read0();
+          __syncwarp();
         };
         if constexpr (EPI == kPairResidual) {
           float v[32];
           sums(c, v);
+          block_free();
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             put(j, __float_as_uint(bf16_round(v[4 * j])), __float_as_uint(bf16_round(v[4 * j + 1])),
@@ -483,6 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
             sums(c + 64 + 32 * h, g);
 #pragma unroll
             for (int j = 0; j < 32; ++j) a[j] = bf16_round(gelu_erf(bf16_round(a[j]))) * bf16_round(g[j]);
+            if (h == 0) block_free();
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               put(4 * h + j, pack_bf16(a[8 * j], a[8 * j + 1]), pack_bf16(a[8 * j + 2], a[8 * j + 3]),
@@ -501,6 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
               v[1][j] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
             }
           }
+          block_free();
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
