@@ -64,7 +64,7 @@ constexpr int kShrinkStages = 4;
 constexpr int kShrinkPitch = kShrinkRanks + 4;
 constexpr int kShrinkXBytes = kShrinkRows * 128, kShrinkABytes = kShrinkCols * 128;
 constexpr int kShrinkPipe = kShrinkStages * (kShrinkXBytes + kShrinkABytes);
-static_assert(kShrinkRows * kShrinkPitch * 4 <= kShrinkPipe, "the partial sums lie over the stages");
+static_assert(kShrinkRows * kShrinkPitch * 4 <= kShrinkPipe, "the parts lie over the stages");
 constexpr int kListInts = 1536;  // write_list's memory
 constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264 + kListInts) * 4 + 128 + 1024;
 
@@ -160,58 +160,38 @@ DEVI void write_list(const LoraParams& p, int row0, int* w) {
   if (tid == 0) out[0] = n;
 }
 
-// The sum of the K slices' parts of a row tile's kept columns, scaled, as V's
-// hi + lo pairs: sixteen lanes take a row (four ranks each), a thread four rows
-// at a time, whose parts are all requested before the first is added.
-// [t0, t1): the rows of this CTA; slot_of(row): the row's adapter, or -1 where
-// another pass or CTA holds it; r0: first rank of the columns.
+// The K slices' parts of the kept columns of this CTA's rows [t0, t1), which
+// every CTA of the cluster sent to recv[slice][row - t0][kShrinkPitch], added
+// in slice order, scaled, as V's hi + lo pairs: sixteen lanes take a row (four
+// ranks each), a thread four rows at a time.  slot_of(row): the row's adapter,
+// or -1 where another pass or CTA holds it; r0: first rank of the columns.
 template <class SlotOf>
-DEVI void write_v(const LoraParams& p, const float* part, int row0, int t0, int t1, int cols, int r0, int split,
+DEVI void write_v(const LoraParams& p, const float* recv, int row0, int t0, int t1, int cols, int r0, int split,
                   SlotOf slot_of) {
   const int c = (threadIdx.x & 15) * 4, r = r0 + c;
   if (c >= cols || (r >> 5) >= p.chunks) return;
-  const uint32_t base = smem_u32(part);
-  for (int first = t0 + (int)(threadIdx.x >> 4); first < t1; first += 32) {
-    float4 sum[4];
-    int slot[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = first + 8 * i;
-      sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      slot[i] = row < t1 ? slot_of(row) : -1;
+  const int per_slice = (t1 - t0) * kShrinkPitch;
+#pragma unroll 4
+  for (int row = t0 + (int)(threadIdx.x >> 4); row < t1; row += 8) {
+    const int slot = slot_of(row);
+    if (slot < 0) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < split; ++k) {
+      const float4 q = *reinterpret_cast<const float4*>(recv + k * per_slice + (row - t0) * kShrinkPitch + c);
+      v.x += q.x;
+      v.y += q.y;
+      v.z += q.z;
+      v.w += q.w;
     }
-    for (int k = 0; k < split; k += 2) {
-      float4 q[4][2];
+    const float f = p.scaling ? p.scaling[slot] : 1.f;
+    const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    float lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (slot[i] >= 0 && k + j < split)
-            q[i][j] = ld_dsmem_f32x4(mapa_shared(base, k + j) + ((first + 8 * i) * kShrinkPitch + c) * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (slot[i] >= 0 && k + j < split) {
-            sum[i].x += q[i][j].x;
-            sum[i].y += q[i][j].y;
-            sum[i].z += q[i][j].z;
-            sum[i].w += q[i][j].w;
-          }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (slot[i] < 0) continue;
-      const float f = p.scaling ? p.scaling[slot[i]] : 1.f;
-      const float x[4] = {sum[i].x * f, sum[i].y * f, sum[i].z * f, sum[i].w * f};
-      float lo[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
-        lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
-      __nv_bfloat16* dst = p.v + ((size_t)(row0 + first + 8 * i) * p.chunks + (r >> 5)) * 64 + (r & 31);
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-      *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-    }
+    for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
+      lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
+    __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
   }
 }
 
@@ -223,14 +203,15 @@ __global__ void __launch_bounds__(192)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sA = smem + ST * kShrinkXBytes;
-  float* part = reinterpret_cast<float*>(smem);               // [128][kShrinkPitch], between passes
+  float* recv = reinterpret_cast<float*>(smem);               // [slice][its rows][kShrinkPitch], between passes
   int* s_ord = reinterpret_cast<int*>(smem + kShrinkPipe);   // [128] each row's place in the list
   int* s_list = s_ord + 128;                                  // [128] distinct adapters
   int* s_tmp = s_list + 128;                                  // [128] + [128] + [4]: number_adapters
   uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264 + kListInts);
   uint64_t* empty = full + ST;
   uint64_t* done = empty + ST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* sent = done + 1;  // the parts of this CTA's rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sent + 1);
   int* s_count = reinterpret_cast<int*>(tmem_slot + 1);
   int* failed = s_count + 1;
   // Everything before this kernel is complete once the wait returns; the
@@ -256,6 +237,7 @@ __global__ void __launch_bounds__(192)
         mbar_init(&empty[s], 1);
       }
       mbar_init(done, 1);
+      mbar_init(sent, 1);
       *failed = 0;
       fence_mbar_init();
       for (int k = 0; k < ST && k < nkb; ++k) load_rows(k, k);
@@ -334,42 +316,61 @@ __global__ void __launch_bounds__(192)
     } else {
       if (!warp_wait(done, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
       tc_fence_after();
-      // a row keeps the columns of its own adapter
-      const int ord = s_ord[tid];
+    }
+    // Every CTA's stages are free: the parts go over them, each row's kept
+    // columns to the CTA that owns the row.
+    const int own_rows = kShrinkRows / split, t0 = rank * own_rows;
+    const int o = warp < 4 ? s_ord[tid] : -1;
+    const bool mine = o >= u && o < u + units;
+    const int owned = __syncthreads_count(mine && tid >= t0 && tid < t0 + own_rows);
+    if (split > 1) {
+      cluster_sync_relaxed();
+      if (tid == 0) mbar_expect_tx(sent, owned * (split - 1) * cols * 4);
+    }
+    if (warp < 4) {
+      const uint32_t to = tid / own_rows;
+      float* here = recv + (rank * own_rows + tid % own_rows) * kShrinkPitch;  // (a row of its own)
+      const uint32_t dst = mapa_shared(smem_u32(here), to);
+      const uint32_t bar = mapa_shared(smem_u32(sent), to);
       for (int a = 0; a < units; ++a) {
-        const bool mine = ord == u + a;
-        if (!__any_sync(0xffffffffu, mine)) continue;
-        for (int c = 0; c < cols; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + a * cols + c, r);
-          tmem_wait_ld();
-          if (mine)
+        if (!__any_sync(0xffffffffu, o == u + a)) continue;
+        const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * cols;
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t r[32];
+          if (cols - c >= 32) {
+            tmem_ld32(acc + c, r);
+          } else {
+            uint32_t h[16];
+            tmem_ld16(acc + c, h);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(part + tid * kShrinkPitch + c + e) =
-                  make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]),
-                              __uint_as_float(r[e + 3]));
+            for (int e = 0; e < 16; ++e) r[e] = h[e];
+          }
+          tmem_wait_ld();
+          if (o == u + a)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < cols) {
+                const float4 v = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]),
+                                             __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+                if (to == (uint32_t)rank)
+                  *reinterpret_cast<float4*>(here + c + e) = v;
+                else
+                  st_async_f32x4(dst + (c + e) * 4, v.x, v.y, v.z, v.w, bar);
+              }
         }
       }
       tc_fence_before();
+      if (split > 1 && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      sync128();
+      write_v(p, recv, row0, t0, t0 + own_rows, cols, group * kShrinkRanks, split, [&](int row) {
+        const int ord = s_ord[row];
+        return ord >= u && ord < u + units ? s_list[ord] : -1;
+      });
     }
-    if (split > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    tc_fence_after();
-    if (warp < 4)
-      write_v(p, part, row0, rank * kShrinkRows / split, (rank + 1) * kShrinkRows / split, cols, group * kShrinkRanks,
-              split, [&](int row) {
-                const int o = s_ord[row];
-                return o >= u && o < u + units ? s_list[o] : -1;
-              });
-    // the partial sums are read; the next pass's copies may take their place
+    // the parts are read; the next pass's copies may take their place
     fence_proxy_async_smem();
-    if (split > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
+    __syncthreads();
+    tc_fence_after();
   }
   tc_fence_before();
   __syncthreads();
@@ -394,8 +395,8 @@ struct FewShrinkCfg {
   static constexpr int STAGES = WIDE ? 3 : 4;
   static constexpr int X_BYTES = kFewRows * 128, A_BYTES = COLS * 128;
   static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
-  static constexpr int PART_BYTES = kFewRows * kShrinkPitch * 4;  // over the stages, between passes
-  static_assert(PART_BYTES <= PIPE_BYTES, "the partial sums fit the pipeline's memory");
+  static constexpr int RECV_BYTES = kFewRows * kShrinkPitch * 4;  // over the stages, between passes
+  static_assert(RECV_BYTES <= PIPE_BYTES, "the parts fit the pipeline's memory");
   static constexpr int SMEM = PIPE_BYTES + (2 * 128 + 264) * 4 + 128 + 1024;
 };
 
@@ -422,13 +423,14 @@ __global__ void __launch_bounds__(160)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sA = smem + ST * C::X_BYTES;
-  float* part = reinterpret_cast<float*>(smem);                 // [64][kShrinkPitch], between passes
+  float* recv = reinterpret_cast<float*>(smem);                 // [slice][its rows][kShrinkPitch], between passes
   int* s_ord = reinterpret_cast<int*>(smem + C::PIPE_BYTES);   // [128] each row's place in the list
   int* s_list = s_ord + 128;                                    // [128] distinct adapters
   int* s_tmp = s_list + 128;                                    // [128] + [128] + [4]: number_adapters
   uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264);
   uint64_t* empty = full + ST;
-  int* s_count = reinterpret_cast<int*>(empty + ST);
+  uint64_t* sent = empty + ST;  // the parts of this CTA's rows
+  int* s_count = reinterpret_cast<int*>(sent + 1);
   int* failed = s_count + 1;
   // Everything before this kernel is complete once the wait returns; the
   // projection launched behind it relies on that (its K blocks do not wait).
@@ -454,6 +456,7 @@ __global__ void __launch_bounds__(160)
         mbar_init(&full[s], 2);   // the rows, the adapters
         mbar_init(&empty[s], 4);  // the warps that compute
       }
+      mbar_init(sent, 1);
       *failed = 0;
       fence_mbar_init();
       for (int k = 0; k < ST && k < nkb; ++k) load_rows(k, k);
@@ -478,8 +481,8 @@ __global__ void __launch_bounds__(160)
       if (!warp_wait(&full[k], 0, limit) && lane == 0) atomicExch(failed, 1);
     }
   Ring<ST> ring;
-  uint32_t g = 0;  // K blocks before this one
-  for (int u = u0; u < u1; u += per) {
+  uint32_t g = 0, pass = 0;  // K blocks and passes before this one
+  for (int u = u0; u < u1; u += per, ++pass) {
     // (after a failure the passes still meet at their barriers)
     const int units = u1 - u < per ? u1 - u : per, ncols = units * cols;
     const int todo = *reinterpret_cast<volatile int*>(failed) ? 0 : nkb;
@@ -499,8 +502,9 @@ __global__ void __launch_bounds__(160)
         }
         __syncwarp();
       }
-    } else {
-      float acc[C::COLS / 8][4];
+    }
+    float acc[C::COLS / 8][4];
+    if (!loader) {
 #pragma unroll
       for (int j = 0; j < C::COLS / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
       for (int k = 0; k < todo; ++k, ring.next()) {
@@ -526,36 +530,46 @@ __global__ void __launch_bounds__(160)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
-      sync128();  // every stage has been read
-      // a row keeps the columns of its own adapter
+    }
+    // Every CTA's stages have been read: the parts go over them, each row's kept
+    // columns to the CTA that owns the row.
+    const int own_rows = kFewRows / split, t0 = rank * own_rows;
+    const int o = !loader && tid < kFewRows ? s_ord[tid] : -1;
+    const int owned = __syncthreads_count(o >= u && o < u + units && tid >= t0 && tid < t0 + own_rows);
+    if (split > 1) {
+      cluster_sync_relaxed();
+      if (tid == 0) mbar_expect_tx(sent, owned * (split - 1) * cols * 4);
+    }
+    if (!loader) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = warp * 16 + (lane >> 2) + 8 * h, unit = s_ord[row] - u;
         if (unit < 0 || unit >= units) continue;
+        const uint32_t to = row / own_rows;
+        float* here = recv + (rank * own_rows + row % own_rows) * kShrinkPitch;  // (a row of its own)
+        const uint32_t dst = mapa_shared(smem_u32(here), to);
+        const uint32_t bar = mapa_shared(smem_u32(sent), to);
 #pragma unroll
         for (int j = 0; j < C::COLS / 8; ++j) {
           const int c = 8 * j + (lane & 3) * 2 - unit * cols;
-          if (c >= 0 && c < cols)
-            *reinterpret_cast<float2*>(part + row * kShrinkPitch + c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+          if (c < 0 || c >= cols) continue;
+          if (to == (uint32_t)rank)
+            *reinterpret_cast<float2*>(here + c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+          else
+            st_async_f32x2(dst + c * 4, acc[j][2 * h], acc[j][2 * h + 1], bar);
         }
       }
+      __syncwarp();
+      if (split > 1 && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      sync128();
+      write_v(p, recv, 0, t0, t0 + own_rows, cols, group * kShrinkRanks, split, [&](int row) {
+        const int ord = s_ord[row];
+        return ord >= u && ord < u + units ? s_list[ord] : -1;
+      });
     }
-    if (split > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    if (!loader)
-      write_v(p, part, 0, rank * kFewRows / split, (rank + 1) * kFewRows / split, cols, group * kShrinkRanks, split,
-              [&](int row) {
-                const int o = s_ord[row];
-                return o >= u && o < u + units ? s_list[o] : -1;
-              });
-    // the partial sums are read; the next pass's copies may take their place
+    // the parts are read; the next pass's copies may take their place
     fence_proxy_async_smem();
-    if (split > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
+    __syncthreads();
   }
   if (tid == 0 && *reinterpret_cast<volatile int*>(failed))
     record_status(p.status ? p.status : &g_op_status, kStatusGemmFullTimeout);
@@ -579,7 +593,7 @@ struct LoraCfg {
   static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int PART_BYTES = BN * 128 * 4;
+  static constexpr int PART_BYTES = 2 * BN * 128 * 4;  // the partial tile, and its tokens' from the other slices
   static constexpr int MAIN_BYTES = PIPE_BYTES > PART_BYTES ? PIPE_BYTES : PART_BYTES;
   static constexpr int LIST_BYTES = (128 + 2 * BN + 264) * 4;  // adapters, their rows, numbering, activation scales
   static constexpr int BAR_BYTES = 256;
@@ -627,10 +641,11 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   uint64_t* vfree = vfull + STAGES;  // the producer found the stage free for an adapter block
   uint64_t* done = vfree + STAGES;
   uint64_t* listed = done + 1;  // the tile's adapter list is in shared memory
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(listed + 1);
+  uint64_t* sent = listed + 1;  // the cluster's parts of this CTA's tokens
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sent + 1);
   uint32_t* failed = tmem_slot + 1;
   int* s_count = reinterpret_cast<int*>(failed + 1);  // distinct adapters, widest span of rows
-  static_assert((4 * STAGES + 2) * 8 + 16 <= C::BAR_BYTES, "barrier block");
+  static_assert((4 * STAGES + 3) * 8 + 16 <= C::BAR_BYTES, "barrier block");
   int* s_list = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [128] distinct adapters
   int* s_span = s_list + 128;                                                 // [BN] first | last << 16 of their rows
   int* s_tmp = s_span + BN;                                                   // [264] number_adapters
@@ -653,6 +668,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     }
     mbar_init(done, 1);
     mbar_init(listed, 1);
+    mbar_init(sent, 1);
     *failed = 0;
     fence_mbar_init();
     prefetch_tensormap(&wmap);
@@ -862,25 +878,29 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   }
   __syncwarp();
 
-  // ---- epilogue: TMEM -> fp32 tile [BN][128] -> cluster reduction -> store
+  // ---- epilogue: the partial tile [token][128] lies over the stages; each
+  // other CTA of the cluster is sent the tokens it stores in one copy, to
+  // recv[slice][token][128] behind the partial tile (its stages are free too
+  // once the relaxed barrier is passed)
   griddep_wait();
+  const int nt = BN / split, t0 = rank * nt;
+  const int stored = max(0, min(p.M - t0, nt));  // its tokens that exist
   if (KIND == kKindFp8)
     for (int i = tid; i < BN; i += C::THREADS) s_scale[i] = i < p.M ? p.a_scale[i] : 0.f;
   if (!warp_wait(done, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
   tc_fence_after();
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
-  {
+  float* recv = part + BN * 128;
+  if (warp < 4) {
     const Share sh = share();
     const bool second = KIND == kKindFp8 && sh.b1 > sh.b0;
-    const int lq = warp & 3;
-    const int lr = lq * 32 + (tid & 31);  // weight row of the tile
-    const uint32_t lane_addr = (uint32_t)(lq * 32) << 16;
+    const int lr = tid;  // weight row of the tile
+    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const float ws = KIND == kKindFp8 && tile_n * 128 + lr < p.N ? p.w_scale[tile_n * 128 + lr] : 1.f;
     constexpr int W = BN < 32 ? 16 : 32;
-    if (warp < 4)
 #pragma unroll 1
-    for (int c = 0; c < BN; c += W) {
+    for (int c = 0; c < BN && c < p.M; c += W) {
       uint32_t r[W], q[W];
       if constexpr (W == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
       if (second) {
@@ -897,49 +917,45 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
         part[(c + j) * 128 + lr] = v;
       }
     }
+    tc_fence_before();
   }
-  tc_fence_before();
+  fence_proxy_async_smem();
   if (split > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
+    cluster_sync_relaxed();  // (every thread of the CTA: its own partial tile is complete too)
+  __syncthreads();
+  if (split > 1) {
+    if (warp == 0 && elect_one()) {
+      mbar_expect_tx(sent, stored * (split - 1) * 512);
+      for (int d = 1; d < split; ++d) {
+        const int to = (rank + d) % split, tokens = min(p.M - to * nt, nt);
+        if (tokens > 0)
+          bulk_copy_to_peer(mapa_shared(smem_u32(recv + rank * nt * 128), to), part + to * nt * 128, tokens * 512,
+                            mapa_shared(smem_u32(sent), to));
+      }
+    }
+    __syncwarp();
+    if (!warp_wait_cluster(sent, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
+  }
   {
-    const int t0 = rank * BN / split, t1 = (rank + 1) * BN / split;
-    const uint32_t part_addr = smem_u32(part);
     const bool rope = tile_n * 128 < p.rope_cols;
     const int pair = rope ? 32 : 64;
     const bool residual = p.epilogue == kEpiResidual;
     const bool plain = p.epilogue == kEpiStore && !rope;
     const bool vec = p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
-    for (int item = tid; item < (t1 - t0) * 16; item += C::THREADS) {
-      const int tl = t0 + (item >> 4);
+    for (int item = tid; item < stored * 16; item += C::THREADS) {
       const int q4 = rope ? ((item >> 3) & 1) * 64 + (item & 7) * 4 : (item & 15) * 4;
-      const int m = tl, n = tile_n * 128 + q4;
-      if (m >= p.M) continue;
-      const int off = tl * 128 + q4;
+      const int m = t0 + (item >> 4), n = tile_n * 128 + q4;
       EpiPre pre;
       if (!plain) pre = epi_prefetch<kKindBf16>(p, m, n, residual, rope);
-      float4 lo, hi;
-      if (split == 1) {
-        lo = *reinterpret_cast<const float4*>(part + off);
-        hi = *reinterpret_cast<const float4*>(part + off + pair);
-      } else {
-        lo = hi = make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 va[8], vb[8];
+      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (u < split) {
-            const uint32_t base = mapa_shared(part_addr, (uint32_t)u);
-            va[u] = ld_dsmem_f32x4(base + off * 4);
-            vb[u] = ld_dsmem_f32x4(base + (off + pair) * 4);
-          }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (u < split) {
-            lo.x += va[u].x; lo.y += va[u].y; lo.z += va[u].z; lo.w += va[u].w;
-            hi.x += vb[u].x; hi.y += vb[u].y; hi.z += vb[u].z; hi.w += vb[u].w;
-          }
-      }
+      for (int u = 0; u < 8; ++u)
+        if (u < split) {
+          const float* src = (u == rank ? part + t0 * 128 : recv + u * nt * 128) + (item >> 4) * 128 + q4;
+          const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + pair);
+          lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
+          hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
+        }
       if (plain) {
         store_quad(p, m, n, lo, vec);
         store_quad(p, m, n + 64, hi, vec);
@@ -950,7 +966,8 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       }
     }
   }
-  if (split > 1) cluster_sync_all();
+
+  if (split > 1) cluster_sync_relaxed();  // every copy out of this CTA's memory has arrived
 
   // ---- teardown: drain copies still in flight after a failure, free TMEM
   if (tid == 0 && *failed) {
@@ -1093,7 +1110,8 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
 
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
                              int split, cudaStream_t stream) {
-  if (p.M < 1 || p.M > bn || p.N < 1 || split < 1 || split > 8 || split > p.kblocks || lp.rows != p.M)
+  if (p.M < 1 || p.M > bn || p.N < 1 || split < 1 || split > 8 || (split & (split - 1)) || split > p.kblocks ||
+      lp.rows != p.M)
     return cudaErrorInvalidValue;
   if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, maps, p, lp, split, stream);
   if (kind == kKindFp8) return dispatch_bn<kKindFp8>(bn, maps, p, lp, split, stream);
