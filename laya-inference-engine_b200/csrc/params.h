@@ -187,6 +187,7 @@ struct RmsNormParams {
   long long ldc;
   float* scale;              // [rows], with codes
   int group;                 // threads that share a row (set by the launcher)
+  int shift, shift_step;     // row r starts (shift + r * shift_step) mod 8 elements into a group of eight (launcher)
 };
 
 struct TailParams {
