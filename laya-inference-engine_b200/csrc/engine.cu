@@ -627,6 +627,7 @@ struct Fwd {
     }
     LoraParams lp{};
     lp.rows = M;
+    lp.out_features = w.N;
     lp.in_features = w.K;
     lp.slots = e->adapter_slots;
     lp.rank = e->adapter_rank;
@@ -636,6 +637,7 @@ struct Fwd {
     lp.x = x;
     lp.ldx = w.K;
     lp.a = ad.a;
+    lp.b = ad.b;
     lp.scaling = ad.scaling;
     lp.v = e->lora_v;
     lp.lists = e->lora_lists;
@@ -650,10 +652,10 @@ struct Fwd {
               slots_map(&maps.a, ad.a, lp.slots, lp.rank, w.K, 64, lora_shrink_box(lp.rank),
                         CU_TENSOR_MAP_SWIZZLE_128B) &&
               rows_map(&maps.w, w.w, w.N, w.K, w.K, esize, wbox) &&
-              rows_map(&maps.x, codes ? (const void*)codes : (const void*)x, M, w.K, w.K, esize, bn) &&
-              slots_map(&maps.b, ad.b, lp.slots, w.N, lp.rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B);
+              rows_map(&maps.x, codes ? (const void*)codes : (const void*)x, M, w.K, w.K, esize, bn);
     if (ok && bnf) {
-      ok = rows_map(&maps.v, lp.v, M, chunks * 64, chunks * 64, 2, 128) &&
+      ok = slots_map(&maps.b, ad.b, lp.slots, w.N, lp.rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B) &&
+           rows_map(&maps.v, lp.v, M, chunks * 64, chunks * 64, 2, 128) &&
            (epi == kEpiResidual ? rows_map(&maps.out, resid, M, p.ldr, p.ldr, 4, 32)
                                 : rows_map(&maps.out, out, M, epi == kEpiGeglu ? w.N / 2 : w.N, ldo, 2, 32));
     }

@@ -49,8 +49,8 @@ cudaError_t launch_gather_rows(float* dst, const float* src, const int* map, int
                                bool pdl);
 cudaError_t launch_tail(const TailParams& p, int batch, cudaStream_t stream, bool pdl);
 cudaError_t launch_token_gather(const TokenGatherParams& p, cudaStream_t stream, bool pdl);
-// Adapters beside a projection (lora.cu): the shrink V = s x A^T, which also
-// lists the adapters of every 256 rows, then the projection that adds V B^T;
+// Adapters beside a projection (lora.cu): the shrink V = s x A^T; for more than
+// 64 rows it also lists the adapters of every 256; then the projection that adds V B^T;
 // launched one behind the other on one stream.  Tensor maps (128-byte swizzle
 // and boxes of 128 bytes of K unless said otherwise):
 struct LoraMaps {

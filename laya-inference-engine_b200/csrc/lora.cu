@@ -3,27 +3,23 @@
 //
 //   out[m] = X[m] W^T + s_a (X[m] A_a^T) B_a^T,   a = index[m / index_div]
 //
-// in two launches.  lora_shrink_kernel computes V[m] = s_a X[m] A_a^T (a few
-// ranks per row).  lora_gemm_kernel is the projection of gemm.cu with its
-// reduction axis lengthened: after the K blocks of W it takes, for every
-// adapter that a row of its token tile uses, the blocks of B_a (TMA) against
-// the rows V of that adapter, zero for the tile's other rows (built in shared
-// memory), into the same TMEM accumulator.  So the adapters cost no pass over
-// the output and no accumulator of their own, a tile whose rows share one
-// adapter pays rank / K of the projection's matrix work, and a tile of single
-// rows with an adapter each pays the bytes of those adapters, which nobody
-// can avoid.
+// in two launches.  The shrink computes V[m] = s_a X[m] A_a^T, a few ranks per
+// row, in one of three kernels: lora_shrink_row_kernel (up to 64 rows, little
+// work: one dot product a warp), lora_shrink_few_kernel (up to 64 rows, mma.sync)
+// and lora_shrink_kernel (tcgen05).  The projection takes the adapters in on the
+// way to its output, so that they cost no pass over it: lora_gemm_kernel (up to 64
+// rows) adds their terms with its K slices, lora_pair_kernel lengthens its
+// reduction axis with the blocks of B_a.
 //
 // The shrink releases the projection once its own inputs are complete, so the
-// projection's K blocks run beside it and only the adapter blocks wait for V.
+// projection's K blocks run beside it and only the adapters wait for V.
 //
 // V is kept as bf16 pairs hi + lo (hi = bf16(v), lo = bf16(v - hi)), about 16
 // bits: a single bf16 V would round the adapter's term once more, by as much as
 // the output's own rounding where the adapter dominates.  A chunk of 32 ranks
-// is one 128-byte row [hi 32 | lo 32] of a swizzled operand tile.
+// is one 128-byte row [hi 32 | lo 32].
 //
-// FP8 projections keep the adapters in bf16: their blocks go to a second
-// accumulator, and the epilogue adds it to the scaled first one.
+// FP8 projections keep the adapters in bf16, added to the scaled products.
 #include "common.cuh"
 #include "params.h"
 #include "launch.h"
@@ -70,6 +66,8 @@ constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264 + kListInts) * 4 + 128 
 
 // The four warps that compute.
 DEVI void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The first four warps of the projection.
+DEVI void sync_low128() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 
 // Numbers the distinct non-negative values of own[] (row h * 128 + thread, 128
 // threads) in order of first appearance: ord[] of each row (-1: none), the
@@ -382,9 +380,9 @@ __global__ void __launch_bounds__(192)
 // ---------------------------------------------------------- shrink, few rows
 // The same for up to 64 rows, which may each bring an adapter of their own:
 // CTAs of 64 rows on mma.sync, whose operands TMA stages, without tensor memory
-// and in little shared memory, so that many share an SM and the projection's
-// CTAs start beside them (64 rows with 64 adapters of rank 16 into 5,248
-// features: 18.6 us with this one in front, 24.3 with the one above).
+// and in little shared memory, so that several share an SM and the projection's
+// CTAs start beside them (64 rows of one adapter of rank 256, K and N 1,024: 15.7
+// us with the projection).
 constexpr int kFewRows = 64;
 
 // WIDE: one adapter of more than 32 ranks at a time; else adapters that
@@ -575,32 +573,231 @@ __global__ void __launch_bounds__(160)
     record_status(p.status ? p.status : &g_op_status, kStatusGemmFullTimeout);
 }
 
+// V of few rows by single dot products: a CTA takes eight ranks of one row, a
+// warp one of them, and reads its adapter's rows for itself.  Nothing is numbered
+// or exchanged and no shared memory is held, so the projection's CTAs all start
+// beside it; rows of one adapter read it again from L2.  Bound by the latency of
+// two dependent loads.
+constexpr int kRowShrinkWarps = 8;
+// Up to 12M products: 16 rows, rank 64, K 2,624 8.9 us with the projection (tiles
+// on mma.sync 12.5); 64, 64, 2,624 14.1 (15.5); 64 rows of one adapter of rank 256,
+// K 1,024, 17.8 (15.7).
+constexpr long long kRowShrinkMacs = 12 << 20;
+
+__global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(const LoraParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int row = blockIdx.y, r = blockIdx.x * kRowShrinkWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int slot = row_adapter(p, row), octets = p.in_features / 8;
+  if (slot < 0) return;
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + (size_t)row * p.ldx);
+  const uint4* a = reinterpret_cast<const uint4*>(p.a + ((size_t)slot * p.rank + r) * p.in_features);
+  float sum = 0.f;
+  for (int c = lane; c < octets; c += 128) {
+    uint4 u[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = v[i] = make_uint4(0, 0, 0, 0);
+      if (c + 32 * i < octets) {
+        u[i] = x[c + 32 * i];
+        v[i] = __ldg(a + c + 32 * i);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t *ui = &u[i].x, *vi = &v[i].x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sum += __uint_as_float(ui[e] << 16) * __uint_as_float(vi[e] << 16);
+        sum += __uint_as_float(ui[e] & 0xffff0000u) * __uint_as_float(vi[e] & 0xffff0000u);
+      }
+    }
+  }
+  sum = warp_sum(sum);
+  if (lane) return;
+  if (p.scaling) sum *= p.scaling[slot];
+  // an infinite (or NaN) value has no remainder
+  const float lo = fabsf(sum) < INFINITY ? sum - bf16_round(sum) : 0.f;
+  __nv_bfloat16* dst = p.v + ((size_t)row * p.chunks + (r >> 5)) * 64 + (r & 31);
+  dst[0] = __float2bfloat16_rn(sum);
+  dst[32] = __float2bfloat16_rn(lo);
+}
+
 // ------------------------------------------------- projection for few rows
 // Up to 64 rows, bound by reading W and the adapters: the tile layout and
 // split-K of gemm.cu (weight rows on the TMEM lanes, rows of X as the MMA's N).
-// An adapter's blocks multiply only the 16-row groups between its first and
-// last row, so 64 single rows with 64 adapters cost as many narrow MMAs; four
-// builder warps prepare the V tiles, each its own blocks, loading the next
-// one's values before they wait for its stage.
-constexpr int kFewBuilders = 4;  // warps, two for each of two stages in turn; half of them divides STAGES, so that
-                                 // each sees every use of its stages
+// The adapters are not blocks of that reduction here.  A CTA stores BN / split
+// rows; four warps add those rows' adapter terms, in fp32, to its own partial
+// tile with mma.sync, while the K slices of the others arrive: per group of
+// eight rows and adapter that they use, 16 ranks a step, the other rows'
+// V zero.  B_a then goes from memory to registers, the first ones before V is
+// there, and nothing waits for a stage.  (As K blocks of the tcgen05 pipeline, V
+// tiles built in shared memory, a block took 0.5 us from its stage's release to
+// its MMAs: 64 rows with 64 adapters of rank 16 into 5,248 features 17.7 us,
+// 10.7 this way.)
+constexpr int kAdapterWarps = 4;
+constexpr int kAdapterAhead = 3;  // (adapter, 16 ranks) steps whose B_a a thread has in registers
 
 template <int BN, int KIND>
 struct LoraCfg {
-  static constexpr int STAGES = 4;
-  static constexpr int THREADS = 64 + 32 * kFewBuilders;
+  static constexpr int STAGES = 3;
+  static constexpr int THREADS = 128 + 32 * kAdapterWarps;
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
   static constexpr int PART_BYTES = 2 * BN * 128 * 4;  // the partial tile, and its tokens' from the other slices
   static constexpr int MAIN_BYTES = PIPE_BYTES > PART_BYTES ? PIPE_BYTES : PART_BYTES;
-  static constexpr int LIST_BYTES = (128 + 2 * BN + 264) * 4;  // adapters, their rows, numbering, activation scales
-  static constexpr int BAR_BYTES = 256;
+  static constexpr int LIST_BYTES = (3 * BN + 4) * 4;  // adapters, activation scales; behind them the adapter terms
+  static constexpr int BAR_BYTES = 128;
   static constexpr int SMEM = MAIN_BYTES + BAR_BYTES + LIST_BYTES + 1024;
-  static constexpr int ACCS = KIND == kKindFp8 ? 2 : 1;
-  static constexpr int TMEM_COLS = BN * ACCS < 32 ? 32 : BN * ACCS;
+  static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
   static constexpr int K_ELEMS = KIND == kKindBf16 ? 64 : 128;
+};
+
+// One group of rows: its two lists' terms are added up in the end.
+__host__ __device__ constexpr int lora_term_lists(int nt) { return nt <= 8 ? 2 : 1; }
+
+// The adapters of `nt` rows from t0 in groups of eight: two lists of pairs (slot;
+// group, and which of its rows use the slot) in group order, s_pair[0..] of the
+// even groups, s_pair[half..] of the odd ones, or of the only group's pairs in
+// turn, their lengths in s_count; one warp.  Their B_a for the features [n0, n0 + 128), contiguous, is on its way to L2.
+DEVI void pair_adapters(const LoraParams& p, int t0, int nt, bool one_group, int n0, int half, int2* s_pair,
+                        int* s_count) {
+  const int lane = threadIdx.x & 31;
+  int n0_list = 0, n1_list = 0;
+  for (int first = 0; first < nt; first += 32) {
+    const int i = first + lane, own = i < nt ? row_adapter(p, t0 + i) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, own) & (0xffu << (lane & 24)), below = (1u << lane) - 1;
+    const bool leads = own >= 0 && __ffs(same) - 1 == lane;
+    const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+    const int odd = one_group ? __popc(leaders & below) & 1 : (lane >> 3) & 1;
+    const unsigned ones = __ballot_sync(0xffffffffu, leads && odd), list = odd ? ones : leaders & ~ones;
+    if (leads) {
+      s_pair[(odd ? half + n1_list : n0_list) + __popc(list & below)] =
+          make_int2(own, i >> 3 | same >> (lane & 24) << 8);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                       p.b + ((size_t)own * p.out_features + n0) * p.rank),
+                   "r"(min(128, p.out_features - n0) * p.rank * 2)
+                   : "memory");
+    }
+    n0_list += __popc(leaders & ~ones);
+    n1_list += __popc(ones);
+  }
+  if (lane == 0) {
+    s_count[0] = n0_list;
+    s_count[1] = n1_list;
+  }
+}
+
+// Four ranks, or zero.
+DEVI uint2 load_ranks_if(const __nv_bfloat16* p, bool in) {
+  uint2 v;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %3, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n"
+      " @p ld.global.cg.v2.u32 {%0,%1}, [%2];\n}\n"
+      : "=r"(v.x), "=r"(v.y)
+      : "l"(p), "r"((int)in));
+  return v;
+}
+DEVI uint2 load_ranks(const __nv_bfloat16* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+// A warp's share of the adapter terms: 64 features from n0 (four m16 tiles) of a
+// list of pairs.  A step is 16 ranks of a pair; a lane holds four consecutive
+// ranks of a row of B_a and of V, which the instruction takes as two pairs: the
+// order of the ranks in its sum is free.  kAdapterAhead steps are in registers,
+// each one's place taken by its successor's loads at once, and the pair of the
+// next loads is read a step before them.  What a step has too many of (ranks,
+// features, steps behind the last) it loads from the nearest valid address and
+// multiplies with a zero V, or adds to a column that is not stored: one warp per
+// scheduler is bound by its instructions, and a predicate for each load doubled
+// them.
+struct AdapterTerms {
+  const LoraParams& p;
+  const int2* s_pair;
+  int pairs, t0, nt;
+  int off[8];  // the lane's rows of B_a
+  uint2 b[kAdapterAhead][8], hi[kAdapterAhead], lo[kAdapterAhead];
+  int group[kAdapterAhead];  // -1 behind the last step
+  int pair_b, k_b, pair_v, k_v;  // the next step to load
+  int slot_b;
+  int2 of_v;
+
+  DEVI void next(int& pair, int& k) const {
+    k += 16;
+    const bool end = k >= p.rank;
+    k = end ? 0 : k;
+    pair += end;
+  }
+  DEVI void load_b(int u) {
+    const int k = min(k_b + 4 * (int)(threadIdx.x & 3), p.rank - 4);
+    const __nv_bfloat16* src = p.b + (size_t)(unsigned)slot_b * ((size_t)p.out_features * p.rank) + k;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[u][j] = load_ranks(src + off[j]);
+    next(pair_b, k_b);
+    slot_b = s_pair[min(pair_b, pairs - 1)].x;
+  }
+  DEVI void load_v(int u) {
+    const int g = (threadIdx.x & 31) >> 2, k = k_v + 4 * (int)(threadIdx.x & 3);
+    const int to = of_v.y & 0xff, row = t0 + to * 8 + g;
+    const bool in = pair_v < pairs && k < p.rank && (of_v.y >> (8 + g) & 1);
+    const __nv_bfloat16* src = p.v + ((size_t)row * p.chunks + (k >> 5)) * 64 + (k & 31);
+    hi[u] = load_ranks_if(src, in);
+    lo[u] = load_ranks_if(src + 32, in);
+    group[u] = pair_v < pairs ? to : -1;
+    next(pair_v, k_v);
+    of_v = s_pair[min(pair_v, pairs - 1)];
+  }
+  // B_a does not wait for V
+  DEVI void start(int n0) {
+    if (pairs == 0) return;
+    const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) off[j] = min(n0 + 8 * j + g, p.out_features - 1) * p.rank;
+    pair_b = k_b = pair_v = k_v = 0;
+    of_v = s_pair[0];
+    slot_b = of_v.x;
+#pragma unroll
+    for (int u = 0; u < kAdapterAhead; ++u) load_b(u);
+  }
+  // out[row][128] = the terms (out: row t0, the warp's first feature)
+  DEVI void store_to(float* out) {
+    if (pairs == 0) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float acc[4][4] = {};
+#pragma unroll
+    for (int u = 0; u < kAdapterAhead; ++u) load_v(u);
+    int now = group[0];
+    while (true) {
+#pragma unroll
+      for (int u = 0; u < kAdapterAhead; ++u) {
+        if (group[u] != now) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (now * 8 + 2 * t + e < nt) {
+              float* dst = out + (now * 8 + 2 * t + e) * 128 + g;
+#pragma unroll
+              for (int f = 0; f < 8; ++f) dst[8 * f] = acc[f >> 1][(f & 1) * 2 + e];
+            }
+          if (group[u] < 0) return;
+          now = group[u];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const uint32_t a[4] = {b[u][m % 4 * 2].x, b[u][m % 4 * 2 + 1].x, b[u][m % 4 * 2].y, b[u][m % 4 * 2 + 1].y};
+          const uint2 v = m < 4 ? hi[u] : lo[u];
+          mma_bf16(acc[m % 4], a, v.x, v.y);
+        }
+        load_b(u);
+        load_v(u);
+      }
+    }
+  }
 };
 
 // Store of one row's four columns n..n+3 (fewer at the matrix's end).
@@ -627,29 +824,24 @@ DEVI void store_quad(const GemmParams& p, int m, int n, float4 v, bool vec) {
 template <int BN, int KIND>
 __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
-                     const __grid_constant__ CUtensorMap bmap, const GemmParams p, const LoraParams lp) {
+                     const GemmParams p, const LoraParams lp) {
   using C = LoraCfg<BN, KIND>;
   constexpr int STAGES = C::STAGES;
-  static_assert(STAGES % (kFewBuilders / 2) == 0 && kFewBuilders == 4, "builder warps and stages");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * C::A_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::MAIN_BYTES);
   uint64_t* empty = full + STAGES;
-  uint64_t* vfull = empty + STAGES;
-  uint64_t* vfree = vfull + STAGES;  // the producer found the stage free for an adapter block
-  uint64_t* done = vfree + STAGES;
-  uint64_t* listed = done + 1;  // the tile's adapter list is in shared memory
-  uint64_t* sent = listed + 1;  // the cluster's parts of this CTA's tokens
+  uint64_t* done = empty + STAGES;
+  uint64_t* sent = done + 1;  // the cluster's parts of this CTA's tokens
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sent + 1);
   uint32_t* failed = tmem_slot + 1;
-  int* s_count = reinterpret_cast<int*>(failed + 1);  // distinct adapters, widest span of rows
-  static_assert((4 * STAGES + 3) * 8 + 16 <= C::BAR_BYTES, "barrier block");
-  int* s_list = reinterpret_cast<int*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [128] distinct adapters
-  int* s_span = s_list + 128;                                                 // [BN] first | last << 16 of their rows
-  int* s_tmp = s_span + BN;                                                   // [264] number_adapters
-  float* s_scale = reinterpret_cast<float*>(s_tmp + 264);                     // [BN] activation scales (fp8)
+  static_assert((2 * STAGES + 2) * 8 + 8 <= C::BAR_BYTES, "barrier block");
+  int2* s_pair = reinterpret_cast<int2*>(smem + C::MAIN_BYTES + C::BAR_BYTES);  // [BN] adapters of the CTA's tokens
+  float* s_scale = reinterpret_cast<float*>(s_pair + BN);                       // [BN] activation scales (fp8)
+  int* s_count = reinterpret_cast<int*>(s_scale + BN);                          // [2], and two unused
+  float* s_terms = reinterpret_cast<float*>(s_count + 4);  // [lists][BN / split][128] adapter terms
 
   const int tid = threadIdx.x, warp = tid >> 5;
   const int tile_n = blockIdx.x;
@@ -657,23 +849,22 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   const int kb0 = (int)((long long)rank * p.kblocks / split);
   const int kb1 = (int)((long long)(rank + 1) * p.kblocks / split);
   const int nkb = kb1 - kb0;
+  const int nt = BN / split, t0 = rank * nt;          // the tokens that this CTA stores,
+  const int stored = max(0, min(p.M - t0, nt));       // those that exist
+  const int lists = lora_term_lists(nt);
   uint32_t* status = p.status ? p.status : &g_op_status;
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&vfull[s], 2);  // the stage's two halves
-      mbar_init(&vfree[s], 1);
     }
     mbar_init(done, 1);
-    mbar_init(listed, 1);
     mbar_init(sent, 1);
     *failed = 0;
     fence_mbar_init();
     prefetch_tensormap(&wmap);
     prefetch_tensormap(&xmap);
-    prefetch_tensormap(&bmap);
   }
   if (warp == 2) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -684,38 +875,16 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   tc_fence_after();
   griddep_launch_dependents();  // only now: the next kernel may allocate tensor memory too
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem2 = tmem + (C::ACCS - 1) * BN;  // the adapters' accumulator
 
   const uint64_t limit = wait_limit(p.wait_limit_us);
   int issued = 0;  // producer warp: loads issued (for the drain on failure)
-  // This rank's share of the tile's adapter blocks (adapter, chunk of 32
-  // ranks), known once `listed` has completed: [b0, b1), `pack` of them in a
-  // stage.  A stage has room for two blocks of half the rows each, which single
-  // rows' adapters are; two at a time keep twice the loads in flight.
-  struct Share {
-    int b0, b1, pack;
-    DEVI int stages() const { return (b1 - b0 + pack - 1) / pack; }
-  };
-  auto share = [&] {
-    const int n = s_count[0] * lp.chunks;
-    return Share{(int)((long long)rank * n / split), (int)((long long)(rank + 1) * n / split),
-                 s_count[1] <= BN / 2 && KIND == kKindBf16 ? 2 : 1};
-  };
-  // Rows [c0, c1) that block b multiplies: whole groups of 16.  The first block
-  // of the FP8 kernels takes every row, which starts their second accumulator.
-  auto span = [&](int b, int b0, int& c0, int& c1) {
-    const int sp = s_span[b / lp.chunks];
-    const bool all = KIND == kKindFp8 && b == b0;
-    c0 = all ? 0 : (sp & 0xffff) & ~15;
-    c1 = all ? BN : ((sp >> 16) + 16) & ~15;
-  };
   auto give_up = [&](uint32_t code) {
     record_status(status, code);
     atomicExch(failed, 1u);
   };
+  // W, X, the adapters and the activation scales do not wait for the shrink:
+  // whatever wrote them was complete before it released this kernel.
   if (warp == 0) {
-    // W, X and B_a do not wait for the shrink: whatever wrote them was
-    // complete before it released this kernel.
     const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
     Ring<STAGES> ring;
     bool ok = true;
@@ -729,26 +898,6 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       }
       __syncwarp();
       issued = i + 1;
-    }
-    ok = ok && warp_wait(listed, 0, limit);
-    if (ok) {
-      const Share sh = share();
-      for (int q = 0; q < sh.stages(); ++q, ring.next()) {
-        const int i = nkb + q, s = ring.s, b = sh.b0 + q * sh.pack, two = sh.pack == 2 && b + 1 < sh.b1;
-        if (i >= STAGES && !(ok = warp_wait(&empty[s], ring.phase ^ 1, limit))) break;
-        if (elect_one()) {
-          mbar_arrive(&vfree[s]);
-          mbar_expect_tx(&full[s], two ? 2 * 128 * 64 : 128 * 64);
-          for (int h = 0; h <= two; ++h)
-            tma_load_3d(sA + s * C::A_BYTES + h * 128 * 64, &bmap, &full[s], ((b + h) % lp.chunks) * 32, tile_n * 128,
-                        s_list[(b + h) / lp.chunks], pol_w);
-        }
-        __syncwarp();
-        issued = i + 1;
-      }
-      // every stage's last release, so that none is in flight at the exit
-      for (int i = issued < STAGES ? 0 : issued - STAGES; ok && i < issued; ++i)
-        ok = warp_wait(&empty[i % STAGES], (i / STAGES) & 1, limit);
     }
     if (!ok && (tid & 31) == 0) give_up(kStatusGemmEmptyTimeout);
   } else if (warp == 1) {
@@ -773,108 +922,26 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       }
       __syncwarp();
     }
-    if (ok && (ok = warp_wait(listed, 0, limit))) {
-      const Share sh = share();
-      for (int q = 0; q < sh.stages(); ++q, ring.next()) {
-        const int s = ring.s, b = sh.b0 + q * sh.pack, two = sh.pack == 2 && b + 1 < sh.b1;
-        if (!(ok = warp_wait(&full[s], ring.phase, limit)) || !(ok = warp_wait(&vfull[s], (q / STAGES) & 1, limit)))
-          break;
-        tc_fence_after();
-        if (elect_one()) {
-          for (int h = 0; h <= two; ++h) {
-            int c0, c1;
-            span(b + h, sh.b0, c0, c1);
-            const uint32_t ad = a0 + s * (C::A_BYTES >> 4) + h * (128 * 64 >> 4);
-            const uint32_t bd = d0 + s * (C::B_BYTES >> 4) + h * (C::B_BYTES / 2 >> 4);
-            const uint32_t id2 = idesc_bf16(128, c1 - c0), acc = tmem2 + c0;
-            umma1_f16<kDesc64, kDesc128>(acc, ad, bd, id2, KIND == kKindBf16 || b > sh.b0);  // hi
-            umma1_f16<kDesc64, kDesc128>(acc, ad, bd + 4, id2, 1);                           // lo
-            if (lp.rank - ((b + h) % lp.chunks) * 32 > 16) {
-              umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 2, id2, 1);
-              umma1_f16<kDesc64, kDesc128>(acc, ad + 2, bd + 6, id2, 1);
-            }
-          }
-          umma_commit(&empty[s]);
-        }
-        __syncwarp();
-      }
-    }
     if (!ok && (tid & 31) == 0) give_up(kStatusGemmFullTimeout);
     if (elect_one()) umma_commit(done);
     __syncwarp();
-  } else if (warp >= 2) {
-    // ---- the tile's adapters in order of first use and the rows each spans
-    // (which do not wait for the shrink), then the V tiles: rows of other
-    // adapters are zero
-    const int bt = tid - 64, lane = tid & 31, bw = bt >> 5;
-    const int own[1] = {bt < BN ? row_adapter(lp, bt) : -1};
-    int ord[1] = {-1};
-    const int n = number_adapters<1>(bt, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
-    int *s_first = s_tmp, *s_last = s_tmp + 128;
+  } else if (warp >= 4) {
+    // ---- the adapter terms of the CTA's tokens
+    const int bt = tid - 128, odd = (warp >> 1) & 1, half = (warp & 1) * 64;
+    for (int i = bt; i < lists * nt * 32; i += 32 * kAdapterWarps)
+      reinterpret_cast<float4*>(s_terms)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (warp == 4) pair_adapters(lp, t0, stored, lists == 2, tile_n * 128, BN / 2, s_pair, s_count);
     sync128();
-    if (bt < n) {
-      s_first[bt] = BN;
-      s_last[bt] = -1;
-    }
-    if (bt == 0) {
-      s_count[0] = n;
-      s_count[1] = 0;
-    }
-    sync128();
-    const unsigned same = __match_any_sync(0xffffffffu, ord[0]);
-    if (ord[0] >= 0 && __ffs(same) - 1 == lane) {  // one lane of a warp's run speaks for it
-      atomicMin(&s_first[ord[0]], bt);
-      atomicMax(&s_last[ord[0]], bt - lane + 31 - __clz(same));
-    }
-    sync128();
-    if (bt < n) {
-      s_span[bt] = s_first[bt] | s_last[bt] << 16;
-      atomicMax(&s_count[1], ((s_last[bt] + 16) & ~15) - (s_first[bt] & ~15));
-    }
-    sync128();
-    if (bt == 0) mbar_arrive(listed);
-    const Share sh = share();
-    const int half = bw & 1, j = lane & 7;  // half of a stage; 16-byte chunk of a V row
-    const int own0 = row_adapter(lp, lane), own1 = BN > 32 ? row_adapter(lp, lane + 32) : -1;
+    AdapterTerms terms{lp, s_pair + odd * (BN / 2), s_count[odd], t0, stored};
+    terms.start(tile_n * 128 + half);
+    // (these warps have no part in the partial tile: they arrive at once, and wait
+    // when they are done)
+    if (split > 1) cluster_arrive_relaxed();
     griddep_wait();  // V
-    // a warp takes its half of every second stage and loads the next block's
-    // values before it waits for the stage
-    for (int q = bw >> 1; q < sh.stages(); q += kFewBuilders / 2) {
-      const int s = (nkb + q) % STAGES, b = sh.b0 + q * sh.pack + half;
-      const bool has = half < sh.pack && b < sh.b1;
-      uint4 v[BN / 4];
-      int c0 = 0, c1 = 0;
-      if (has) {
-        const int c = b % lp.chunks, slot = s_list[b / lp.chunks];
-        const int ksteps = lp.rank - c * 32 > 16 ? 2 : 1;
-        span(b, sh.b0, c0, c1);
-#pragma unroll
-        for (int u = 0; u < BN / 4; ++u) {
-          const int row = c0 + u * 4 + (lane >> 3);
-          const int o0 = __shfl_sync(0xffffffffu, own0, row & 31), o1 = __shfl_sync(0xffffffffu, own1, row & 31);
-          v[u] = make_uint4(0, 0, 0, 0);
-          if (row < c1 && (row < 32 ? o0 : o1) == slot && (j & 3) < 2 * ksteps)
-            v[u] = *reinterpret_cast<const uint4*>(lp.v + ((size_t)row * lp.chunks + c) * 64 + j * 8);
-        }
-      }
-      // (the builders cannot wait on `empty` themselves: they have not followed
-      // its phases through the K blocks, and a parity names every second one)
-      if (!warp_wait(&vfree[s], (q / STAGES) & 1, limit)) {
-        if (lane == 0) give_up(kStatusGemmEmptyTimeout);
-        break;
-      }
-      if (has) {
-        uint8_t* dst = sB + s * C::B_BYTES + half * (C::B_BYTES / 2);
-#pragma unroll
-        for (int u = 0; u < BN / 4; ++u) {
-          const int row = u * 4 + (lane >> 3);
-          if (c0 + row < c1) *reinterpret_cast<uint4*>(dst + sw128_offset(row, j)) = v[u];
-        }
-        fence_proxy_async_smem();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[s]);
-    }
+    terms.store_to(s_terms + odd * (lists - 1) * nt * 128 + half);
+    if (split > 1) cluster_wait();
+  } else if (KIND == kKindFp8) {
+    for (int i = tid - 64; i < BN; i += 64) s_scale[i] = i < p.M ? p.a_scale[i] : 0.f;
   }
   __syncwarp();
 
@@ -882,60 +949,49 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   // other CTA of the cluster is sent the tokens it stores in one copy, to
   // recv[slice][token][128] behind the partial tile (its stages are free too
   // once the relaxed barrier is passed)
-  griddep_wait();
-  const int nt = BN / split, t0 = rank * nt;
-  const int stored = max(0, min(p.M - t0, nt));  // its tokens that exist
-  if (KIND == kKindFp8)
-    for (int i = tid; i < BN; i += C::THREADS) s_scale[i] = i < p.M ? p.a_scale[i] : 0.f;
-  if (!warp_wait(done, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
-  tc_fence_after();
-  __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
   float* recv = part + BN * 128;
   if (warp < 4) {
-    const Share sh = share();
-    const bool second = KIND == kKindFp8 && sh.b1 > sh.b0;
+    if (!warp_wait(done, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
+    tc_fence_after();
+    if (KIND == kKindFp8) sync_low128();  // the activation scales
     const int lr = tid;  // weight row of the tile
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const float ws = KIND == kKindFp8 && tile_n * 128 + lr < p.N ? p.w_scale[tile_n * 128 + lr] : 1.f;
     constexpr int W = BN < 32 ? 16 : 32;
 #pragma unroll 1
     for (int c = 0; c < BN && c < p.M; c += W) {
-      uint32_t r[W], q[W];
+      uint32_t r[W];
       if constexpr (W == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
-      if (second) {
-        if constexpr (W == 32) tmem_ld32(tmem2 + lane_addr + c, q); else tmem_ld16(tmem2 + lane_addr + c, q);
-      }
       tmem_wait_ld();
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         float v = __uint_as_float(r[j]);
-        if (KIND == kKindFp8) {
-          v = (v * s_scale[c + j]) * ws;
-          if (second) v += __uint_as_float(q[j]);
-        }
+        if (KIND == kKindFp8) v = (v * s_scale[c + j]) * ws;
         part[(c + j) * 128 + lr] = v;
       }
     }
     tc_fence_before();
-  }
-  fence_proxy_async_smem();
-  if (split > 1)
-    cluster_sync_relaxed();  // (every thread of the CTA: its own partial tile is complete too)
-  __syncthreads();
-  if (split > 1) {
-    if (warp == 0 && elect_one()) {
-      mbar_expect_tx(sent, stored * (split - 1) * 512);
-      for (int d = 1; d < split; ++d) {
-        const int to = (rank + d) % split, tokens = min(p.M - to * nt, nt);
-        if (tokens > 0)
-          bulk_copy_to_peer(mapa_shared(smem_u32(recv + rank * nt * 128), to), part + to * nt * 128, tokens * 512,
-                            mapa_shared(smem_u32(sent), to));
+    fence_proxy_async_smem();
+    if (split > 1) {
+      cluster_arrive_relaxed();
+      cluster_wait();  // every CTA's stages are free
+      sync_low128();   // and this one's partial tile complete
+      if (warp == 0 && elect_one()) {
+        mbar_expect_tx(sent, stored * (split - 1) * 512);
+        for (int d = 1; d < split; ++d) {
+          const int to = (rank + d) % split, tokens = min(p.M - to * nt, nt);
+          if (tokens > 0)
+            bulk_copy_to_peer(mapa_shared(smem_u32(recv + rank * nt * 128), to), part + to * nt * 128, tokens * 512,
+                              mapa_shared(smem_u32(sent), to));
+        }
       }
+      __syncwarp();
     }
-    __syncwarp();
-    if (!warp_wait_cluster(sent, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
+    griddep_wait();  // what wrote or read the output
   }
+  if (split > 1 && !warp_wait_cluster(sent, 0, limit) && (tid & 31) == 0) give_up(kStatusGemmDoneTimeout);
+  __syncthreads();
   {
     const bool rope = tile_n * 128 < p.rope_cols;
     const int pair = rope ? 32 : 64;
@@ -948,14 +1004,14 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       EpiPre pre;
       if (!plain) pre = epi_prefetch<kKindBf16>(p, m, n, residual, rope);
       float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (u < split) {
-          const float* src = (u == rank ? part + t0 * 128 : recv + u * nt * 128) + (item >> 4) * 128 + q4;
-          const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + pair);
-          lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
-          hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
-        }
+      const int at = (item >> 4) * 128 + q4;
+#pragma unroll 2
+      for (int u = 0; u < split + lists; ++u) {  // the slices in order, then the adapters
+        const float* src = (u >= split ? s_terms + (u - split) * nt * 128 : u == rank ? part + t0 * 128 : recv + u * nt * 128) + at;
+        const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + pair);
+        lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
+        hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
+      }
       if (plain) {
         store_quad(p, m, n, lo, vec);
         store_quad(p, m, n + 64, hi, vec);
@@ -995,7 +1051,7 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
   {
     std::lock_guard<std::mutex> lock(mu);
     if (!(ready >> dev & 1)) {
-      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM + BN * 512);  // (split 1: the most)
       if (err != cudaSuccess) return err;
       ready |= uint64_t(1) << dev;
     }
@@ -1003,7 +1059,7 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.N + 127) / 128, 1, split);
   cfg.blockDim = dim3(C::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.dynamicSmemBytes = C::SMEM + lora_term_lists(BN / split) * (BN / split) * 512;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1017,7 +1073,7 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
     cfg.numAttrs = 2;
   }
   cfg.attrs = attrs;
-  return cudaLaunchKernelEx(&cfg, kern, maps.w, maps.x, maps.b, p, lp);
+  return cudaLaunchKernelEx(&cfg, kern, maps.w, maps.x, p, lp);
 }
 
 template <int KIND>
@@ -1054,7 +1110,9 @@ cudaError_t launch_shrink(const void* kern, int smem, int threads, dim3 grid, co
     attrs[cfg.numAttrs].val.clusterDim.y = 1;
     attrs[cfg.numAttrs++].val.clusterDim.z = grid.z;
   }
-  void* args[] = {const_cast<CUtensorMap*>(&maps.rows), const_cast<CUtensorMap*>(&maps.a), const_cast<LoraParams*>(&p)};
+  void* with_maps[] = {const_cast<CUtensorMap*>(&maps.rows), const_cast<CUtensorMap*>(&maps.a),
+                       const_cast<LoraParams*>(&p)};
+  void** args = smem ? with_maps : with_maps + 2;  // (the kernel without shared memory takes no tensor map)
   return cudaLaunchKernelExC(&cfg, kern, args);
 }
 
@@ -1063,7 +1121,7 @@ cudaError_t launch_shrink(const void* kern, int smem, int threads, dim3 grid, co
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                cudaStream_t stream, bool pdl) {
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
-      p.index_div < 1 || !p.lists)
+      p.index_div < 1 || (!p.lists && lora_shrink_rows(p.rows) == kShrinkRows))
     return cudaErrorInvalidValue;
   constexpr int kWide = FewShrinkCfg<true>::SMEM, kSlim = FewShrinkCfg<false>::SMEM;
   static std::mutex mu;
@@ -1084,6 +1142,9 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
   }
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, kblocks = (p.in_features + 63) / 64;
   if (lora_shrink_rows(p.rows) == kFewRows) {
+    if ((long long)p.rows * p.rank * p.in_features <= kRowShrinkMacs)
+      return launch_shrink((const void*)lora_shrink_row_kernel, 0, 32 * kRowShrinkWarps,
+                           dim3(p.rank / kRowShrinkWarps, p.rows, 1), maps, p, stream, pdl);
     // The adapters are spread first, then K, up to three CTAs per SM.
     const bool wide = p.rank > 32;
     const int per = (wide ? 64 : 32) / lora_shrink_box(p.rank), room = std::max(1, 3 * sm_count / groups);
@@ -1111,7 +1172,7 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
                              int split, cudaStream_t stream) {
   if (p.M < 1 || p.M > bn || p.N < 1 || split < 1 || split > 8 || (split & (split - 1)) || split > p.kblocks ||
-      lp.rows != p.M)
+      lp.rows != p.M || !lp.b)
     return cudaErrorInvalidValue;
   if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, maps, p, lp, split, stream);
   if (kind == kKindFp8) return dispatch_bn<kKindFp8>(bn, maps, p, lp, split, stream);

@@ -61,8 +61,11 @@ DEVI bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
 // Cluster barrier that orders nothing (a release at cluster scope takes over a
 // microsecond): used where the CTAs only tell each other that their memory may
 // be written; the data comes as st.async, counted by an mbarrier.
+DEVI void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+DEVI void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 DEVI void cluster_sync_relaxed() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+  cluster_arrive_relaxed();
+  cluster_wait();
 }
 // Shared memory of this CTA to another CTA's of the cluster (16-byte multiples),
 // counted on a barrier there.

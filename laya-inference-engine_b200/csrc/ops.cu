@@ -188,12 +188,14 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
                         CU_TENSOR_MAP_SWIZZLE_128B) &&
               rows_map(&maps.w, a->weight, N, K, a->weight_stride, wsize, wbox) &&
               rows_map(&maps.x, operand, M, K, ldo, wsize, plan.bnf ? 128 : plan.bn) &&
-              slots_map(&maps.b, a->lora_b, a->slots, N, a->rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B) &&
-              (!plan.bnf || rows_map(&maps.v, workspace, M, chunks * 64, chunks * 64, 2, 128)) &&
+              (!plan.bnf ||
+               (slots_map(&maps.b, a->lora_b, a->slots, N, a->rank, 32, wbox, CU_TENSOR_MAP_SWIZZLE_64B) &&
+                rows_map(&maps.v, workspace, M, chunks * 64, chunks * 64, 2, 128))) &&
               (!tma_out || rows_map(&maps.out, a->out, M, N, a->out_stride, 2, 32));
     if (!ok) return reject("a tensor map was rejected");
     LoraParams lp{};
     lp.rows = M;
+    lp.out_features = a->out_features;
     lp.in_features = K;
     lp.slots = a->slots;
     lp.rank = a->rank;
@@ -203,6 +205,7 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     lp.x = static_cast<const __nv_bfloat16*>(a->x);
     lp.ldx = a->x_stride;
     lp.a = static_cast<const __nv_bfloat16*>(a->lora_a);
+    lp.b = static_cast<const __nv_bfloat16*>(a->lora_b);
     lp.scaling = a->scaling;
     lp.v = static_cast<__nv_bfloat16*>(workspace);
     GemmParams p{};

@@ -161,9 +161,11 @@ struct LoraParams {
   const __nv_bfloat16* x;    // [rows][ldx]
   long long ldx;
   const __nv_bfloat16* a;    // [slots][rank][in_features]
+  const __nv_bfloat16* b;    // [slots][out_features][rank]
+  int out_features;
   const float* scaling;      // [slots] or null (1)
   __nv_bfloat16* v;          // [rows][chunks][64]
-  int* lists;                // [ceil(rows / 256)][kLoraListInts]
+  int* lists;                // [ceil(rows / 256)][kLoraListInts]; unused up to 64 rows
   uint32_t* status;          // device-visible status word, or null
 };
 
