@@ -56,13 +56,13 @@ namespace {
 constexpr int kShrinkRows = 128;
 constexpr int kShrinkRanks = 64;   // ranks of an adapter in one CTA
 constexpr int kShrinkCols = 256;   // columns of one pass
-constexpr int kShrinkStages = 4;
-constexpr int kShrinkPitch = kShrinkRanks + 4;
-constexpr int kShrinkXBytes = kShrinkRows * 128, kShrinkABytes = kShrinkCols * 128;
-constexpr int kShrinkPipe = kShrinkStages * (kShrinkXBytes + kShrinkABytes);
-static_assert(kShrinkRows * kShrinkPitch * 4 <= kShrinkPipe, "the parts lie over the stages");
+constexpr int kShrinkXBytes = kShrinkRows * 128;
+constexpr int kShrinkPipe = 4 * (kShrinkXBytes + kShrinkCols * 128);
+constexpr int kShrinkStages = 10;  // at most
+constexpr int kShrinkFirst = 4;  // row blocks requested before the adapters are known
+static_assert(2 * kShrinkRows * (kShrinkRanks + 4) * 4 <= kShrinkPipe, "the parts lie over the stages");
 constexpr int kListInts = 1536;  // write_list's memory
-constexpr int kShrinkSmem = kShrinkPipe + (2 * 128 + 264 + kListInts) * 4 + 128 + 1024;
+constexpr int kShrinkSmem = kShrinkPipe + (3 * 128 + 264 + kListInts) * 4 + 256 + 1024;
 
 // The four warps that compute.
 DEVI void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -71,9 +71,9 @@ DEVI void sync_low128() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 
 // Numbers the distinct non-negative values of own[] (row h * 128 + thread, 128
 // threads) in order of first appearance: ord[] of each row (-1: none), the
-// values in s_list, their count returned (tid: 0..127).  A warp's leaders look for their
-// value among the earlier warps' leaders only, so a tile of long runs costs a
-// few steps.  s_tmp, s_entry: H * 128 ints (16-byte aligned); s_cnt: H * 4.
+// values in s_list, their count returned (tid: 0..127).  A warp's leaders look for
+// their value among the earlier warps' leaders only, so a tile of long runs costs
+// a few steps.  s_tmp, s_entry: H * 128 ints (16-byte aligned); s_cnt: H * 8.
 template <int H>
 DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_list, int* s_tmp, int* s_entry,
                          int* s_cnt) {
@@ -89,21 +89,25 @@ DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_lis
     __syncwarp();
     entry[h] = own[h] >= 0 && lead[h] == lane ? h * 128 + warp * 32 + __popc(leaders & below) : -1;
     if (entry[h] >= 0) s_tmp[entry[h]] = own[h];
+    if (lane == 0) s_cnt[h * 4 + warp] = __popc(leaders);
   }
   sync128();
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     seen[h] = H * 128;
     if (entry[h] >= 0)
-      for (int j = 0; j < h * 128 + warp * 32; j += 4) {
-        const int4 v = *reinterpret_cast<const int4*>(s_tmp + j);
-        if (v.w == own[h]) seen[h] = min(seen[h], j + 3);
-        if (v.z == own[h]) seen[h] = min(seen[h], j + 2);
-        if (v.y == own[h]) seen[h] = min(seen[h], j + 1);
-        if (v.x == own[h]) seen[h] = min(seen[h], j);
-      }
+#pragma unroll 1
+      for (int w = 0; w < h * 4 + warp && seen[h] == H * 128; ++w)
+#pragma unroll 1
+        for (int j = w * 32; j < w * 32 + s_cnt[w]; j += 4) {
+          const int4 v = *reinterpret_cast<const int4*>(s_tmp + j);
+          if (v.w == own[h]) seen[h] = j + 3;
+          if (v.z == own[h]) seen[h] = j + 2;
+          if (v.y == own[h]) seen[h] = j + 1;
+          if (v.x == own[h]) seen[h] = j;
+        }
     firsts[h] = __ballot_sync(0xffffffffu, entry[h] >= 0 && seen[h] == H * 128);
-    if (lane == 0) s_cnt[h * 4 + warp] = __popc(firsts[h]);
+    if (lane == 0) s_cnt[H * 4 + h * 4 + warp] = __popc(firsts[h]);
   }
   sync128();
   int n = 0;
@@ -115,7 +119,7 @@ DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_lis
       s_entry[entry[h]] = ord[h];
       s_list[ord[h]] = own[h];
     }
-    n += s_cnt[w];
+    n += s_cnt[H * 4 + w];
   }
   sync128();
 #pragma unroll
@@ -128,11 +132,10 @@ DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_lis
 }
 
 // Writes the list of the 256 rows from row0 for the projection: count, adapters,
-// and each one's first and last row.  128 threads; `w`: 1536 ints of shared memory.
-DEVI void write_list(const LoraParams& p, int row0, int* w) {
+// and each one's first and last row.  own: adapters of rows tid and 128 + tid; 128 threads; `w`: 1536 ints of shared memory.
+DEVI void write_list(const LoraParams& p, int row0, const int (&own)[2], int* w) {
   const int tid = threadIdx.x, lane = tid & 31;
-  int own[2], ord[2] = {-1, -1};
-  for (int h = 0; h < 2; ++h) own[h] = row_adapter(p, row0 + 128 * h + tid);
+  int ord[2] = {-1, -1};
   int *s_list = w, *s_span = w + 256;
   const int n = number_adapters<2>(tid, own, ord, s_list, w + 768, w + 1024, w + 1280);
   for (int j = tid; j < n; j += 128) {
@@ -158,30 +161,44 @@ DEVI void write_list(const LoraParams& p, int row0, int* w) {
   if (tid == 0) out[0] = n;
 }
 
-// The K slices' parts of the kept columns of this CTA's rows [t0, t1), which
-// every CTA of the cluster sent to recv[slice][row - t0][kShrinkPitch], added
-// in slice order, scaled, as V's hi + lo pairs: sixteen lanes take a row (four
-// ranks each), a thread four rows at a time.  slot_of(row): the row's adapter,
-// or -1 where another pass or CTA holds it; r0: first rank of the columns.
-template <class SlotOf>
-DEVI void write_v(const LoraParams& p, const float* recv, int row0, int t0, int t1, int cols, int r0, int split,
-                  SlotOf slot_of) {
-  const int c = (threadIdx.x & 15) * 4, r = r0 + c;
+// The K slices' parts of a CTA's rows lie in part[row][pitch]; those that another
+// CTA of the cluster owns go there in one copy, to recv[slice][its rows][pitch].
+// (As st.async of each thread, 16 bytes each, this took 4 us.)  One thread; the
+// parts are complete and fenced, the peers' memory free.
+DEVI void send_parts(const float* part, float* recv, int own_rows, int pitch, int rank, int split, uint64_t* sent) {
+  const uint32_t bytes = own_rows * pitch * 4;
+  mbar_expect_tx(sent, bytes * (split - 1));
+  for (int d = 1; d < split; ++d) {
+    const int to = (rank + d) % split;
+    bulk_copy_to_peer(mapa_shared(smem_u32(recv + rank * own_rows * pitch), to), part + to * own_rows * pitch, bytes,
+                      mapa_shared(smem_u32(sent), to));
+  }
+}
+
+// The parts of the kept columns of this CTA's rows [t0, t1) added in slice
+// order, scaled, as V's hi + lo pairs, four ranks a thread.  taken(row): this pass of this CTA has the row's adapter; s_factor: the
+// rows' scaling; r0: first rank of the columns.
+template <class Taken>
+DEVI void write_v(const LoraParams& p, const float* part, const float* recv, const float* s_factor, int row0, int t0,
+                  int t1, int cols, int pitch, int r0, int rank, int split, Taken taken) {
+  const int shift = cols <= 16 ? 2 : cols <= 32 ? 3 : 4;  // lanes of a row
+  const int c = (threadIdx.x & ((1 << shift) - 1)) * 4, r = r0 + c;
   if (c >= cols || (r >> 5) >= p.chunks) return;
-  const int per_slice = (t1 - t0) * kShrinkPitch;
-#pragma unroll 4
-  for (int row = t0 + (int)(threadIdx.x >> 4); row < t1; row += 8) {
-    const int slot = slot_of(row);
-    if (slot < 0) continue;
+  const int per_slice = (t1 - t0) * pitch;
+#pragma unroll 1
+  for (int row = t0 + (int)(threadIdx.x >> shift); row < t1; row += 128 >> shift) {
+    if (!taken(row)) continue;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
     for (int k = 0; k < split; ++k) {
-      const float4 q = *reinterpret_cast<const float4*>(recv + k * per_slice + (row - t0) * kShrinkPitch + c);
+      const float* src = k == rank ? part + row * pitch : recv + k * per_slice + (row - t0) * pitch;
+      const float4 q = *reinterpret_cast<const float4*>(src + c);
       v.x += q.x;
       v.y += q.y;
       v.z += q.z;
       v.w += q.w;
     }
-    const float f = p.scaling ? p.scaling[slot] : 1.f;
+    const float f = s_factor[row];
     const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
     float lo[4];
 #pragma unroll
@@ -199,12 +216,12 @@ __global__ void __launch_bounds__(192)
   constexpr int ST = kShrinkStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sX = smem;
-  uint8_t* sA = smem + ST * kShrinkXBytes;
-  float* recv = reinterpret_cast<float*>(smem);               // [slice][its rows][kShrinkPitch], between passes
+  uint8_t* sX = smem;  // row blocks from the front, adapter blocks from the back
+  float* part = reinterpret_cast<float*>(smem);               // over the stages, between passes
   int* s_ord = reinterpret_cast<int*>(smem + kShrinkPipe);   // [128] each row's place in the list
   int* s_list = s_ord + 128;                                  // [128] distinct adapters
-  int* s_tmp = s_list + 128;                                  // [128] + [128] + [4]: number_adapters
+  float* s_factor = reinterpret_cast<float*>(s_list + 128);   // [128] each row's scaling
+  int* s_tmp = s_list + 256;                                  // [128] + [128] + [4]: number_adapters
   uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264 + kListInts);
   uint64_t* empty = full + ST;
   uint64_t* done = empty + ST;
@@ -228,6 +245,8 @@ __global__ void __launch_bounds__(192)
     mbar_expect_tx(&full[s], kShrinkXBytes);
     tma_load_2d(sX + s * kShrinkXBytes, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
   };
+  const bool lists = row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1;  // this CTA writes the list of 256 rows
+  int of_list[2] = {-1, -1};
   if (warp == 4) {
     if (elect_one()) {
       for (int s = 0; s < ST; ++s) {
@@ -238,7 +257,7 @@ __global__ void __launch_bounds__(192)
       mbar_init(sent, 1);
       *failed = 0;
       fence_mbar_init();
-      for (int k = 0; k < ST && k < nkb; ++k) load_rows(k, k);
+      for (int k = 0; k < kShrinkFirst && k < nkb; ++k) load_rows(k, k);
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -247,9 +266,13 @@ __global__ void __launch_bounds__(192)
   } else {
     // ---- the tile's adapters in order of first use (the rows are on their way)
     const int own[1] = {row_adapter(p, row0 + tid)};
+    of_list[0] = own[0];
+    if (lists) of_list[1] = row_adapter(p, row0 + 128 + tid);
     int ord[1] = {-1};
+    const float factor = own[0] >= 0 && p.scaling ? __ldg(p.scaling + own[0]) : 1.f;
     const int n = number_adapters<1>(tid, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
     s_ord[tid] = ord[0];
+    s_factor[tid] = factor;
     if (tid == 0) *s_count = n;
   }
   tc_fence_before();
@@ -260,40 +283,55 @@ __global__ void __launch_bounds__(192)
   const int n = *s_count;
   const int u0 = (int)((long long)slice * n / slices), u1 = (int)((long long)(slice + 1) * n / slices);
   const int per = kShrinkCols / cols;  // adapters of one pass
+  const int pitch = cols + 4;
+  float* recv = part + kShrinkRows * pitch;
   if (warp == 4 && u0 == u1)           // no adapter here: the rows still land before the exit
-    for (int k = 0; k < ST && k < nkb; ++k) {
+    for (int k = 0; k < kShrinkFirst && k < nkb; ++k) {
       if (elect_one()) mbar_arrive(&full[k]);
       __syncwarp();
       if (!warp_wait(&full[k], 0, limit) && lane == 0) atomicExch(failed, 1);
     }
   // the projection's list of 256 rows, while the first K blocks are on their way
-  if (warp < 4 && row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1) write_list(p, row0, s_tmp + 264);
-  Ring<ST> ring;
+  if (warp < 4 && lists) write_list(p, row0, of_list, s_tmp + 264);
+  // as many stages as the memory holds with the columns of the largest pass
+  const int a_bytes = (min(per, u1 - u0) * cols * 128 + 1023) & ~1023;
+  const int stages = min(ST, kShrinkPipe / (kShrinkXBytes + a_bytes));
+  auto adapters_of = [&](int s) { return smem + kShrinkPipe - (s + 1) * a_bytes; };
+  struct {
+    int s = 0;
+    uint32_t phase = 0;
+    DEVI void next(int n) {
+      if (++s == n) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+  } ring;
   uint32_t g = 0, pass = 0;  // K blocks and passes before this one
   for (int u = u0; u < u1; u += per, ++pass) {
     // (after a failure the passes still meet at their barriers)
     const int units = u1 - u < per ? u1 - u : per;
     const int todo = *reinterpret_cast<volatile int*>(failed) ? 0 : nkb;
     if (warp == 4) {
-      for (int k = 0; k < todo; ++k, ++g, ring.next()) {
+      for (int k = 0; k < todo; ++k, ++g, ring.next(stages)) {
         const int s = ring.s;
-        if (g >= ST && !warp_wait(&empty[s], ring.phase ^ 1, limit)) {
+        if ((int)g >= stages && !warp_wait(&empty[s], ring.phase ^ 1, limit)) {
           if (lane == 0) atomicExch(failed, 1);
           break;
         }
         if (elect_one()) {
-          if (g >= ST || (int)g >= nkb) load_rows(s, k);  // (the first ones were requested above)
+          if (g >= kShrinkFirst || (int)g >= nkb) load_rows(s, k);  // (the first ones were requested above)
           mbar_expect_tx(&full[s], units * cols * 128);
           for (int a = 0; a < units; ++a)
-            tma_load_3d(sA + s * kShrinkABytes + a * cols * 128, &amap, &full[s], (kb0 + k) * 64, group * kShrinkRanks,
+            tma_load_3d(adapters_of(s) + a * cols * 128, &amap, &full[s], (kb0 + k) * 64, group * kShrinkRanks,
                         s_list[u + a], pol);
         }
         __syncwarp();
       }
     } else if (warp == 5) {
       const uint32_t idesc = idesc_bf16(128, units * cols);
-      const uint32_t x0 = desc_lo(smem_u32(sX)), a0 = desc_lo(smem_u32(sA));
-      for (int k = 0; k < todo; ++k, ring.next()) {
+      const uint32_t x0 = desc_lo(smem_u32(sX));
+      for (int k = 0; k < todo; ++k, ring.next(stages)) {
         const int s = ring.s;
         if (!warp_wait(&full[s], ring.phase, limit)) {
           if (lane == 0) atomicExch(failed, 1);
@@ -301,7 +339,7 @@ __global__ void __launch_bounds__(192)
         }
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t xd = x0 + s * (kShrinkXBytes >> 4), ad = a0 + s * (kShrinkABytes >> 4);
+          const uint32_t xd = x0 + s * (kShrinkXBytes >> 4), ad = desc_lo(smem_u32(adapters_of(s)));
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             umma1_f16<kDesc128, kDesc128>(tmem, xd + 2 * e, ad + 2 * e, idesc, (k | e) != 0);
@@ -315,58 +353,43 @@ __global__ void __launch_bounds__(192)
       if (!warp_wait(done, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
       tc_fence_after();
     }
-    // Every CTA's stages are free: the parts go over them, each row's kept
-    // columns to the CTA that owns the row.
+    // The parts go over the stages, whose blocks have all been read: each row's
+    // kept columns.
     const int own_rows = kShrinkRows / split, t0 = rank * own_rows;
-    const int o = warp < 4 ? s_ord[tid] : -1;
-    const bool mine = o >= u && o < u + units;
-    const int owned = __syncthreads_count(mine && tid >= t0 && tid < t0 + own_rows);
-    if (split > 1) {
-      cluster_sync_relaxed();
-      if (tid == 0) mbar_expect_tx(sent, owned * (split - 1) * cols * 4);
-    }
     if (warp < 4) {
-      const uint32_t to = tid / own_rows;
-      float* here = recv + (rank * own_rows + tid % own_rows) * kShrinkPitch;  // (a row of its own)
-      const uint32_t dst = mapa_shared(smem_u32(here), to);
-      const uint32_t bar = mapa_shared(smem_u32(sent), to);
+      const int o = s_ord[tid];
+      float* here = part + tid * pitch;
       for (int a = 0; a < units; ++a) {
         if (!__any_sync(0xffffffffu, o == u + a)) continue;
         const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * cols;
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          if (cols - c >= 32) {
-            tmem_ld32(acc + c, r);
-          } else {
-            uint32_t h[16];
-            tmem_ld16(acc + c, h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) r[e] = h[e];
-          }
+        for (int c = 0; c < cols; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(acc + c, r);
           tmem_wait_ld();
           if (o == u + a)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c + e < cols) {
-                const float4 v = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]),
-                                             __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
-                if (to == (uint32_t)rank)
-                  *reinterpret_cast<float4*>(here + c + e) = v;
-                else
-                  st_async_f32x4(dst + (c + e) * 4, v.x, v.y, v.z, v.w, bar);
-              }
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(here + c + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
         }
       }
       tc_fence_before();
-      if (split > 1 && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      fence_proxy_async_smem();
       sync128();
-      write_v(p, recv, row0, t0, t0 + own_rows, cols, group * kShrinkRanks, split, [&](int row) {
-        const int ord = s_ord[row];
-        return ord >= u && ord < u + units ? s_list[ord] : -1;
-      });
     }
-    // the parts are read; the next pass's copies may take their place
+    if (split > 1) {
+      cluster_sync_relaxed();  // every CTA's stages are free
+      if (warp == 0 && elect_one()) send_parts(part, recv, own_rows, pitch, rank, split, sent);
+      __syncwarp();
+      if (warp < 4 && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      __syncwarp();
+      cluster_arrive_relaxed();
+    }
+    if (warp < 4)
+      write_v(p, part, recv, s_factor, row0, t0, t0 + own_rows, cols, pitch, group * kShrinkRanks, rank, split,
+              [&](int row) { return s_ord[row] >= u && s_ord[row] < u + units; });
+    // the parts are read, here and by the copies; the next pass may take their place
     fence_proxy_async_smem();
+    if (split > 1) cluster_wait();
     __syncthreads();
     tc_fence_after();
   }
@@ -393,9 +416,8 @@ struct FewShrinkCfg {
   static constexpr int STAGES = WIDE ? 3 : 4;
   static constexpr int X_BYTES = kFewRows * 128, A_BYTES = COLS * 128;
   static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
-  static constexpr int RECV_BYTES = kFewRows * kShrinkPitch * 4;  // over the stages, between passes
-  static_assert(RECV_BYTES <= PIPE_BYTES, "the parts fit the pipeline's memory");
-  static constexpr int SMEM = PIPE_BYTES + (2 * 128 + 264) * 4 + 128 + 1024;
+  static_assert(2 * kFewRows * (kShrinkRanks + 4) * 4 <= PIPE_BYTES, "the parts fit the pipeline's memory");
+  static constexpr int SMEM = PIPE_BYTES + (3 * 128 + 264) * 4 + 128 + 1024;
 };
 
 DEVI void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -421,10 +443,11 @@ __global__ void __launch_bounds__(160)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sA = smem + ST * C::X_BYTES;
-  float* recv = reinterpret_cast<float*>(smem);                 // [slice][its rows][kShrinkPitch], between passes
+  float* part = reinterpret_cast<float*>(smem);                // over the stages, between passes
   int* s_ord = reinterpret_cast<int*>(smem + C::PIPE_BYTES);   // [128] each row's place in the list
   int* s_list = s_ord + 128;                                    // [128] distinct adapters
-  int* s_tmp = s_list + 128;                                    // [128] + [128] + [4]: number_adapters
+  float* s_factor = reinterpret_cast<float*>(s_list + 128);    // [128] each row's scaling
+  int* s_tmp = s_list + 256;                                    // [128] + [128] + [4]: number_adapters
   uint64_t* full = reinterpret_cast<uint64_t*>(s_tmp + 264);
   uint64_t* empty = full + ST;
   uint64_t* sent = empty + ST;  // the parts of this CTA's rows
@@ -464,14 +487,18 @@ __global__ void __launch_bounds__(160)
     // ---- the tile's adapters in order of first use (the rows are on their way)
     const int own[1] = {tid < kFewRows ? row_adapter(p, tid) : -1};
     int ord[1] = {-1};
+    const float factor = own[0] >= 0 && p.scaling ? __ldg(p.scaling + own[0]) : 1.f;
     const int n = number_adapters<1>(tid, own, ord, s_list, s_tmp, s_tmp + 128, s_tmp + 256);
     s_ord[tid] = ord[0];
+    s_factor[tid] = factor;
     if (tid == 0) *s_count = n;
   }
   __syncthreads();
   const int n = *s_count;
   const int u0 = (int)((long long)slice * n / slices), u1 = (int)((long long)(slice + 1) * n / slices);
   const int per = C::COLS / cols;  // adapters of one pass
+  const int pitch = cols + 4;
+  float* recv = part + kFewRows * pitch;
   if (loader && u0 == u1)          // no adapter here: the rows still land before the exit
     for (int k = 0; k < ST && k < nkb; ++k) {
       if (elect_one()) mbar_arrive(&full[k]);
@@ -529,44 +556,40 @@ __global__ void __launch_bounds__(160)
         if (lane == 0) mbar_arrive(&empty[s]);
       }
     }
-    // Every CTA's stages have been read: the parts go over them, each row's kept
-    // columns to the CTA that owns the row.
+    // The parts go over the stages, once all of them have been read: each row's
+    // kept columns.
     const int own_rows = kFewRows / split, t0 = rank * own_rows;
-    const int o = !loader && tid < kFewRows ? s_ord[tid] : -1;
-    const int owned = __syncthreads_count(o >= u && o < u + units && tid >= t0 && tid < t0 + own_rows);
-    if (split > 1) {
-      cluster_sync_relaxed();
-      if (tid == 0) mbar_expect_tx(sent, owned * (split - 1) * cols * 4);
-    }
+    __syncthreads();
     if (!loader) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = warp * 16 + (lane >> 2) + 8 * h, unit = s_ord[row] - u;
         if (unit < 0 || unit >= units) continue;
-        const uint32_t to = row / own_rows;
-        float* here = recv + (rank * own_rows + row % own_rows) * kShrinkPitch;  // (a row of its own)
-        const uint32_t dst = mapa_shared(smem_u32(here), to);
-        const uint32_t bar = mapa_shared(smem_u32(sent), to);
 #pragma unroll
         for (int j = 0; j < C::COLS / 8; ++j) {
           const int c = 8 * j + (lane & 3) * 2 - unit * cols;
-          if (c < 0 || c >= cols) continue;
-          if (to == (uint32_t)rank)
-            *reinterpret_cast<float2*>(here + c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-          else
-            st_async_f32x2(dst + c * 4, acc[j][2 * h], acc[j][2 * h + 1], bar);
+          if (c >= 0 && c < cols)
+            *reinterpret_cast<float2*>(part + row * pitch + c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
         }
       }
       __syncwarp();
-      if (split > 1 && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      fence_proxy_async_smem();
       sync128();
-      write_v(p, recv, 0, t0, t0 + own_rows, cols, group * kShrinkRanks, split, [&](int row) {
-        const int ord = s_ord[row];
-        return ord >= u && ord < u + units ? s_list[ord] : -1;
-      });
     }
-    // the parts are read; the next pass's copies may take their place
+    if (split > 1) {
+      cluster_sync_relaxed();  // every CTA's stages are free
+      if (warp == 0 && elect_one()) send_parts(part, recv, own_rows, pitch, rank, split, sent);
+      __syncwarp();
+      if (!loader && !warp_wait_cluster(sent, pass & 1, limit) && lane == 0) atomicExch(failed, 1);
+      __syncwarp();
+      cluster_arrive_relaxed();
+    }
+    if (!loader)
+      write_v(p, part, recv, s_factor, 0, t0, t0 + own_rows, cols, pitch, group * kShrinkRanks, rank, split,
+              [&](int row) { return s_ord[row] >= u && s_ord[row] < u + units; });
+    // the parts are read, here and by the copies; the next pass may take their place
     fence_proxy_async_smem();
+    if (split > 1) cluster_wait();
     __syncthreads();
   }
   if (tid == 0 && *reinterpret_cast<volatile int*>(failed))

@@ -60,7 +60,7 @@ DEVI bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
 
 // Cluster barrier that orders nothing (a release at cluster scope takes over a
 // microsecond): used where the CTAs only tell each other that their memory may
-// be written; the data comes as st.async, counted by an mbarrier.
+// be written; the data comes as bulk copies, counted by an mbarrier.
 DEVI void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 DEVI void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 DEVI void cluster_sync_relaxed() {
@@ -72,11 +72,6 @@ DEVI void cluster_sync_relaxed() {
 DEVI void bulk_copy_to_peer(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "r"(smem_u32(src)), "r"(bytes), "r"(bar)
-               : "memory");
-}
-DEVI void st_async_f32x2(uint32_t addr, float a, float b, uint32_t bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(addr), "f"(a),
-               "f"(b), "r"(bar)
                : "memory");
 }
 // mbar_wait_cluster by a whole warp, with one verdict for its lanes.
