@@ -648,9 +648,10 @@ struct Fwd {
     p.tma_epilogue = bnf ? 1 : 0;
     const int wbox = bnf ? bnf / 2 : 128;
     LoraMaps maps{};
-    bool ok = rows_map(&maps.rows, x, M, w.K, w.K, 2, lora_shrink_rows(M)) &&
-              slots_map(&maps.a, ad.a, lp.slots, lp.rank, w.K, 64, lora_shrink_box(lp.rank),
-                        CU_TENSOR_MAP_SWIZZLE_128B) &&
+    bool ok = (lora_shrink_by_row(M, lp.rank, w.K) ||
+               (rows_map(&maps.rows, x, M, w.K, w.K, 2, lora_shrink_rows(M)) &&
+                slots_map(&maps.a, ad.a, lp.slots, lp.rank, w.K, 64, lora_shrink_box(lp.rank),
+                          CU_TENSOR_MAP_SWIZZLE_128B))) &&
               rows_map(&maps.w, w.w, w.N, w.K, w.K, esize, wbox) &&
               rows_map(&maps.x, codes ? (const void*)codes : (const void*)x, M, w.K, w.K, esize, bn);
     if (ok && bnf) {

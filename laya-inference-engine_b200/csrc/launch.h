@@ -65,6 +65,13 @@ struct LoraMaps {
 // projection_ctas: CTAs of the projection behind it (launch_lora_pairs' grid), 0 for few rows.
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                cudaStream_t stream, bool pdl);
+// Whether the shrink takes single dot products, without maps.rows and maps.a: up
+// to 64 rows, and 12M products: 16 rows, rank 64, K 2,624 8.9 us with the
+// projection (tiles on mma.sync 12.5); 64, 64, 2,624 14.1 (15.5); 64 rows of one
+// adapter of rank 256, K 1,024, 17.8 (15.7).
+inline bool lora_shrink_by_row(int rows, int rank, int in_features) {
+  return rows <= 64 && (long long)rows * rank * in_features <= 12 << 20;
+}
 // Rows, and ranks of one adapter, in a CTA of the shrink.
 inline int lora_shrink_rows(int rows) { return rows <= 64 ? 64 : 128; }
 __host__ __device__ inline int lora_shrink_box(int rank) { return rank < 64 ? (rank + 15) / 16 * 16 : 64; }

@@ -602,10 +602,6 @@ __global__ void __launch_bounds__(160)
 // beside it; rows of one adapter read it again from L2.  Bound by the latency of
 // two dependent loads.
 constexpr int kRowShrinkWarps = 8;
-// Up to 12M products: 16 rows, rank 64, K 2,624 8.9 us with the projection (tiles
-// on mma.sync 12.5); 64, 64, 2,624 14.1 (15.5); 64 rows of one adapter of rank 256,
-// K 1,024, 17.8 (15.7).
-constexpr long long kRowShrinkMacs = 12 << 20;
 
 __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(const LoraParams p) {
   griddep_wait();
@@ -1165,7 +1161,7 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
   }
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, kblocks = (p.in_features + 63) / 64;
   if (lora_shrink_rows(p.rows) == kFewRows) {
-    if ((long long)p.rows * p.rank * p.in_features <= kRowShrinkMacs)
+    if (lora_shrink_by_row(p.rows, p.rank, p.in_features))
       return launch_shrink((const void*)lora_shrink_row_kernel, 0, 32 * kRowShrinkWarps,
                            dim3(p.rank / kRowShrinkWarps, p.rows, 1), maps, p, stream, pdl);
     // The adapters are spread first, then K, up to three CTAs per SM.

@@ -8,7 +8,9 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
@@ -180,6 +182,13 @@ void run_rms_norm(const Tensor& x, const Tensor* weight, double eps, const Tenso
   check("rms_norm", laya_b200_rms_norm(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
 }
 
+// A new tensor beside x, without the dispatcher's microsecond (a tensor that is
+// not on a GPU is refused later).
+Tensor empty_beside(const Tensor& x, at::IntArrayRef sizes, ScalarType type) {
+  if (!x.is_cuda()) return at::empty(sizes, x.options().dtype(type).requires_grad(false));
+  return at::detail::empty_cuda(sizes, type, x.device(), c10::nullopt);
+}
+
 // rms_norm(x, weight, eps, residual, out, dtype)
 PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -198,7 +207,7 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (given && (given->sizes() != x.sizes() || (typed && given->scalar_type() != type)))
     refuse("out must have x's shape " + shape_of(x.sizes()) + (typed ? " and be of dtype" : ""));
   if (!given && type != kBF16 && type != kF32) refuse("dtype must be torch.bfloat16 or torch.float32");
-  const Tensor out = given ? *given : at::empty(x.sizes(), x.options().dtype(type).requires_grad(false));
+  const Tensor out = given ? *given : empty_beside(x, x.sizes(), type);
   run_rms_norm(x, weight, eps, residual, &out, given != nullptr, nullptr, nullptr);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
@@ -215,10 +224,9 @@ PyObject* py_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   const int keep = PyObject_IsTrue(args[4]);
   if (keep < 0) throw python_error();
   if (x.dim() < 1) refuse("x must be a tensor of rows");
-  const auto plain = x.options().requires_grad(false);
-  const Tensor codes = at::empty(x.sizes(), plain.dtype(kE4M3));
-  const Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), plain.dtype(kF32));
-  const Tensor y = keep ? at::empty(x.sizes(), plain) : Tensor();
+  const Tensor codes = empty_beside(x, x.sizes(), kE4M3);
+  const Tensor scale = empty_beside(x, x.sizes().slice(0, x.dim() - 1), kF32);
+  const Tensor y = keep ? empty_beside(x, x.sizes(), x.scalar_type()) : Tensor();
   run_rms_norm(x, weight, eps, residual, keep ? &y : nullptr, false, &codes, &scale);
   PyObject* out = PyTuple_New(keep ? 3 : 2);
   if (!out) throw python_error();
@@ -271,7 +279,7 @@ PyObject* py_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (k % (fp8 ? 16 : 8)) refuse(std::string("in_features must be a multiple of ") + (fp8 ? "16" : "8"));
   const at::Device dev =
       device_of({&x, codes, code_scale, &weight, weight_scale, &la, &lb, &index, scaling, bias, given});
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
   a.out_stride = n;
   if (given) {
@@ -279,8 +287,7 @@ PyObject* py_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.out_stride = rows_of("out", *given, {kBF16}, n).stride;
     disjoint("out", *given, {&x, codes, code_scale, &weight, weight_scale, &la, &lb, &index, scaling, bias});
   }
-  const auto plain = x.options().requires_grad(false);
-  const Tensor out = given ? *given : at::empty(shape, plain);
+  const Tensor out = given ? *given : empty_beside(x, shape, kBF16);
   if (rx.rows == 0 || n == 0) return THPVariable_Wrap(out);
   a.rows = narrow("rows", rx.rows);
   a.in_features = narrow("in_features", k);
@@ -305,8 +312,8 @@ PyObject* py_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   size_t bytes = 0;
   check("lora_linear", laya_b200_lora_workspace(&a, &bytes));
   // the caching allocator hands this memory to later work of this stream only
-  const Tensor work = at::empty({(int64_t)bytes}, plain.dtype(ScalarType::Byte));
-  check("lora_linear", laya_b200_lora_linear(&a, work.data_ptr(), bytes,
+  const c10::DataPtr work = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+  check("lora_linear", laya_b200_lora_linear(&a, work.get(), bytes,
                                              c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
