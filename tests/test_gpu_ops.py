@@ -406,3 +406,129 @@ def test_gpu_refusals():
         ops.rms_norm(x, residual=torch.zeros(64, device=DEV).expand(4, 64))
     with pytest.raises(ValueError):
         ops.rms_norm(x[:2], out=x[1:3])
+
+
+@pytest.mark.parametrize("m, k, n, rank, slots", [
+    (64, 64, 40000, 24, 64),    # more feature tiles than CTAs: K is not split, a CTA stores all rows
+    (64, 512, 300, 256, 64), (8, 1024, 512, 136, 8), (13, 2624, 130, 248, 2),
+    (9, 20000, 72, 8, 3),       # a long K
+    (64, 4096, 130, 64, 9), (50, 2624, 257, 104, 50),  # V by tiles instead of single products
+    (48, 1024, 1024, 8, 200), (5, 16, 1, 16, 2), (64, 16, 8, 8, 1),
+    (65, 512, 40, 256, 65), (256, 64, 129, 16, 200), (257, 80, 300, 40, 2), (1023, 4096, 520, 48, 31),
+])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_lora_linear_corners(m, k, n, rank, slots, fp8):
+    if fp8:
+        k = (k + 15) // 16 * 16
+    s = make(m * 3 + n, m, k, n, rank, slots, fp8, bias=n % 2 == 0)
+    check_lora(s, (torch.arange(m, device=DEV) % slots).to(torch.int32))
+    check_lora(s, runs(m + 1, m, max(1, min(m, 9)), slots))
+    check_lora(s, torch.tensor([slots - 1, -1, 0], dtype=torch.int32, device=DEV).repeat(m)[:(m + 6) // 7].contiguous(),
+               per=7)
+    assert ops.op_status() == 0
+
+
+@pytest.mark.parametrize("m", [1, 7, 24, 64])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_few_requests_do_not_reach_each_other(m, fp8):
+    k, n, rank, slots = 256, 300, 24, 5
+    s = make(50 + m, m, k, n, rank, slots, fp8)
+    index = (torch.arange(m, device=DEV) // 3 % slots).to(torch.int32)
+    clean = check_lora(s, index)
+    x = s["x"].clone()
+    x[m // 2, 3], x[m - 1, 100] = float("nan"), float("inf")
+    got = call(dict(s, x=x), index)
+    others = torch.ones(m, dtype=torch.bool, device=DEV)
+    others[[m // 2, m - 1]] = False
+    assert torch.equal(got[others], clean[others]) and not got[~others].isfinite().any()
+    a = s["a"].clone()
+    a[0, 5, 9] = float("nan")
+    got = call(dict(s, a=a), index)
+    assert torch.equal(got[index != 0], clean[index != 0]) and got[index == 0].isnan().all()
+    # a slot that nobody uses may hold anything
+    a, b = s["a"].clone(), s["b"].clone()
+    a[1], b[1] = float("nan"), float("inf")
+    other = torch.where(index == 1, 2, index).to(torch.int32)
+    assert torch.equal(call(dict(s, a=a, b=b), other), call(s, other))
+
+
+@pytest.mark.parametrize("rows, d", [(3, 16), (40, 17), (33, 23), (1, 31), (700, 127), (2001, 435), (64, 1001),
+                                     (900, 2623), (700, 4001), (5, 4099), (300, 16383), (10000, 129)])
+@pytest.mark.parametrize("x_type, r_type", [(BF16, F32), (BF16, BF16), (F32, None)])
+def test_rms_norm_odd_rows(rows, d, x_type, r_type):
+    """Rows off the 16-byte boundaries: all buffers alike, and not."""
+    g = gen(rows + d)
+    w = 1 + randn(g, d + 1, std=0.2)
+    for lo, ld in ((0, d), (0, d + d % 8), (3, (d + 15) // 8 * 8 + 5)):
+        x = randn(g, rows, ld + lo, dtype=x_type)[:, lo:lo + d]
+        if r_type is None:
+            r = None
+        else:
+            whole = randn(g, rows, ld + lo, std=3.0, dtype=r_type)
+            r, before = whole[:, lo:lo + d], whole.clone()
+        _, ref = rms_reference(x, w[:d], 1e-5, r)
+        out = torch.full((rows, ld + lo), 9.0, dtype=x_type, device=DEV)
+        ops.rms_norm(x, w[:d], residual=r, out=out[:, lo:lo + d])
+        assert ((out[:, lo:lo + d].double() - ref).abs() <= y_bound(ref, x_type)).all()
+        assert (out[:, :lo] == 9).all() and (out[:, lo + d:] == 9).all()
+        if r is not None:
+            before[:, lo:lo + d] = (before[:, lo:lo + d].float() + x.float()).to(r_type)
+            assert torch.equal(whole, before)
+        # the others' rows at distances of their own, a weight off its boundary
+        check_rms(x, w[1:], None if r is None else r.clone(), True)
+
+
+def test_two_streams_at_once():
+    """Calls of every kernel in flight on two streams."""
+    cases = [make(60 + i, *c) for i, c in enumerate(
+        ((1, 512, 256, 16, 2), (64, 1024, 512, 256, 6), (64, 512, 1000, 16, 64), (300, 512, 520, 64, 7)))]
+    cases += [make(70, 48, 512, 256, 16, 5, True), make(71, 500, 512, 256, 16, 5, True)]
+    index = [(torch.arange(s["x"].shape[0], device=DEV) % s["a"].shape[0]).to(torch.int32) for s in cases]
+    refs = [check_lora(s, i) for s, i in zip(cases, index)]
+    norm = [ops.rms_norm(r) for r in refs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], ([], [])
+    for _ in range(10):
+        for j, (s, i) in enumerate(zip(cases, index)):
+            for side, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    y = call(s, i)
+                    got[side].append((j, y, ops.rms_norm(y)))
+    torch.cuda.synchronize()
+    for j, y, z in got[0] + got[1]:
+        assert torch.equal(y, refs[j]) and torch.equal(z, norm[j])
+    assert ops.op_status() == 0
+
+
+FIRST_IN_CAPTURE = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from laya_b200 import ops
+which = sys.argv[2]
+dev = torch.device("cuda")
+m = {"few": 5, "tiles": 64, "many": 300, "rms": 5}[which]
+x = torch.ones(m, 1024, dtype=torch.bfloat16, device=dev)
+w = torch.ones(64, 1024, dtype=torch.bfloat16, device=dev)
+a = torch.ones(2, 256, 1024, dtype=torch.bfloat16, device=dev)
+b = torch.ones(2, 64, 256, dtype=torch.bfloat16, device=dev)
+i = torch.zeros(m, dtype=torch.int32, device=dev)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.rms_norm(x) if which == "rms" else ops.lora_linear(x, w, a, b, i)
+g.replay()
+torch.cuda.synchronize()
+want = 1.0 if which == "rms" else 1024 + 256 * 1024
+assert (y.float() - want).abs().max() <= want / 256, y
+"""
+
+
+@pytest.mark.parametrize("which", ["few", "tiles", "many", "rms"])
+def test_first_call_inside_a_capture(which):
+    import pathlib
+    import subprocess
+    import sys
+
+    root = str(pathlib.Path(ops.__file__).resolve().parents[1])
+    done = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE, root, which], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
