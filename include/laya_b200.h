@@ -224,7 +224,7 @@ typedef struct laya_b200_rms_norm_args {
   void* residual;            /* updated in place to h (rounded to its type), or NULL: h = x */
   int64_t residual_stride;
   const float* weight;       /* [columns] or NULL (1) */
-  void* y;                   /* or NULL */
+  void* y;                   /* or NULL; may be x itself with x's type and stride */
   int64_t y_stride;
   void* codes;               /* e4m3, or NULL */
   int64_t codes_stride;

@@ -611,6 +611,7 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
   if (slot < 0) return;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + (size_t)row * p.ldx);
   const uint4* a = reinterpret_cast<const uint4*>(p.a + ((size_t)slot * p.rank + r) * p.in_features);
+  const float factor = p.scaling ? __ldg(p.scaling + slot) : 1.f;
   float sum = 0.f;
   for (int c = lane; c < octets; c += 128) {
     uint4 u[4], v[4];
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
   }
   sum = warp_sum(sum);
   if (lane) return;
-  if (p.scaling) sum *= p.scaling[slot];
+  sum *= factor;
   // an infinite (or NaN) value has no remainder
   const float lo = fabsf(sum) < INFINITY ? sum - bf16_round(sum) : 0.f;
   __nv_bfloat16* dst = p.v + ((size_t)row * p.chunks + (r >> 5)) * 64 + (r & 31);

@@ -82,8 +82,8 @@ bool lora_plan(const laya_b200_lora_args* a, int sm_count, LoraPlan* plan) {
   const int rows = a->rows > 0 ? a->rows : 1;
   auto align_up = [](size_t x) { return (x + 255) / 256 * 256; };
   plan->v_bytes = align_up((size_t)rows * ((a->rank + 31) / 32) * 128);
-  plan->list_bytes = align_up((size_t)((rows + 255) / 256) * kLoraListInts * sizeof(int));
   plan->bnf = lora_pair_plan(plan->kind, rows, a->out_features, sm_count);
+  plan->list_bytes = plan->bnf ? align_up((size_t)((rows + 255) / 256) * kLoraListInts * sizeof(int)) : 0;
   if (!plan->bnf) lora_few_plan(rows, a->out_features, plan->kblocks, sm_count, &plan->bn, &plan->split);
   return true;
 }
@@ -221,7 +221,7 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     p.bias = static_cast<const __nv_bfloat16*>(a->bias);
     p.a_scale = a->code_scale;
     p.w_scale = a->weight_scale;
-    lp.lists = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
+    if (plan.bnf) lp.lists = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t err = launch_lora_shrink(
         maps, lp, sms, plan.bnf ? lora_pair_ctas(M, N, plan.bnf, sms) : 0, st, true);
