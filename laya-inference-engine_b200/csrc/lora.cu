@@ -50,9 +50,11 @@ namespace {
 // keeps the columns of its own, so that no row sees another adapter's values.
 // The K slices of a cluster are added through distributed shared memory in
 // rank order.  Bound by the loads (rows and adapters once each) and, for few
-// rows, by the latency of two dependent loads and the exchange.  (On mma.sync,
-// small enough to share its SM with the projection, it took 15 us for 8,192
-// rows and 41 K blocks: too few bytes in flight.)
+// rows, by latency: 8,192 rows of K 2,624 with 16 adapters of rank 16 take 12 us,
+// 7.5 of them the loads at the memory's rate; 777 of K 1,000 6.3 us, 1.9 until the
+// adapters are numbered, 2.5 for the loads, 1.9 for the exchange and V.  (On
+// mma.sync, small enough to share its SM with the projection, 15 us for 8,192 rows
+// and 41 K blocks: too few bytes in flight.)
 constexpr int kShrinkRows = 128;
 constexpr int kShrinkRanks = 64;   // ranks of an adapter in one CTA
 constexpr int kShrinkCols = 256;   // columns of one pass
@@ -132,7 +134,8 @@ DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_lis
 }
 
 // Writes the list of the 256 rows from row0 for the projection: count, adapters,
-// and each one's first and last row.  own: adapters of rows tid and 128 + tid; 128 threads; `w`: 1536 ints of shared memory.
+// and each one's first and last row.  own: adapters of rows tid and 128 + tid;
+// 128 threads; `w`: 1536 ints of shared memory.
 DEVI void write_list(const LoraParams& p, int row0, const int (&own)[2], int* w) {
   const int tid = threadIdx.x, lane = tid & 31;
   int ord[2] = {-1, -1};
@@ -163,8 +166,7 @@ DEVI void write_list(const LoraParams& p, int row0, const int (&own)[2], int* w)
 
 // The K slices' parts of a CTA's rows lie in part[row][pitch]; those that another
 // CTA of the cluster owns go there in one copy, to recv[slice][its rows][pitch].
-// (As st.async of each thread, 16 bytes each, this took 4 us.)  One thread; the
-// parts are complete and fenced, the peers' memory free.
+// One thread; the parts are complete and fenced, the peers' memory free.
 DEVI void send_parts(const float* part, float* recv, int own_rows, int pitch, int rank, int split, uint64_t* sent) {
   const uint32_t bytes = own_rows * pitch * 4;
   mbar_expect_tx(sent, bytes * (split - 1));
@@ -175,9 +177,17 @@ DEVI void send_parts(const float* part, float* recv, int own_rows, int pitch, in
   }
 }
 
+// What bf16(v) leaves of v; nothing where it is infinite or NaN.
+DEVI float v_remainder(float v) {
+  const float hi = bf16_round(v);
+  return fabsf(hi) < INFINITY ? v - hi : 0.f;
+}
+
 // The parts of the kept columns of this CTA's rows [t0, t1) added in slice
-// order, scaled, as V's hi + lo pairs, four ranks a thread.  taken(row): this pass of this CTA has the row's adapter; s_factor: the
-// rows' scaling; r0: first rank of the columns.
+// order, scaled, as V's hi + lo pairs, four ranks a thread.  taken(row): this
+// pass of this CTA has the row's adapter; s_factor: the rows' scaling; r0: first
+// rank of the columns.  Its loops are not unrolled: four rows at a time took a
+// microsecond more.
 template <class Taken>
 DEVI void write_v(const LoraParams& p, const float* part, const float* recv, const float* s_factor, int row0, int t0,
                   int t1, int cols, int pitch, int r0, int rank, int split, Taken taken) {
@@ -202,8 +212,7 @@ DEVI void write_v(const LoraParams& p, const float* part, const float* recv, con
     const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
     float lo[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)  // an infinite (or NaN) value has no remainder
-      lo[k] = fabsf(x[k]) < INFINITY ? x[k] - bf16_round(x[k]) : 0.f;
+    for (int k = 0; k < 4; ++k) lo[k] = v_remainder(x[k]);
     __nv_bfloat16* dst = p.v + ((size_t)(row0 + row) * p.chunks + (r >> 5)) * 64 + (r & 31);
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
     *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
@@ -636,8 +645,7 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
   sum = warp_sum(sum);
   if (lane) return;
   sum *= factor;
-  // an infinite (or NaN) value has no remainder
-  const float lo = fabsf(sum) < INFINITY ? sum - bf16_round(sum) : 0.f;
+  const float lo = v_remainder(sum);
   __nv_bfloat16* dst = p.v + ((size_t)row * p.chunks + (r >> 5)) * 64 + (r & 31);
   dst[0] = __float2bfloat16_rn(sum);
   dst[32] = __float2bfloat16_rn(lo);
@@ -647,14 +655,17 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
 // Up to 64 rows, bound by reading W and the adapters: the tile layout and
 // split-K of gemm.cu (weight rows on the TMEM lanes, rows of X as the MMA's N).
 // The adapters are not blocks of that reduction here.  A CTA stores BN / split
-// rows; four warps add those rows' adapter terms, in fp32, to its own partial
-// tile with mma.sync, while the K slices of the others arrive: per group of
-// eight rows and adapter that they use, 16 ranks a step, the other rows'
-// V zero.  B_a then goes from memory to registers, the first ones before V is
-// there, and nothing waits for a stage.  (As K blocks of the tcgen05 pipeline, V
-// tiles built in shared memory, a block took 0.5 us from its stage's release to
-// its MMAs: 64 rows with 64 adapters of rank 16 into 5,248 features 17.7 us,
-// 10.7 this way.)
+// rows, and four warps compute those rows' adapter terms with mma.sync, in fp32,
+// while the K blocks and the exchange of the slices run: per group of eight rows
+// and adapter that they use, 16 ranks a step, the other rows' V zero.  B_a goes
+// from memory to registers, the first of it before V is there, and the terms wait
+// for no stage.  Measured, 64 rows with 64 adapters of rank 16 into 5,248 features:
+// 10.7 us, 8.5 with one adapter, 8.2 with none (the bytes take 3.5): the two
+// launches' chain, then 0.3 us a step, which is the loads' latency over the three
+// steps that registers hold.  (As K blocks of the tcgen05 pipeline, V tiles built
+// in shared memory, 17.7 us: a block took 0.5 us from its stage's release to its
+// MMAs.)  Three stages: the shrink's CTAs then leave room for every CTA of this
+// kernel beside them (with four, the last ones started 4 us late).
 constexpr int kAdapterWarps = 4;
 constexpr int kAdapterAhead = 3;  // (adapter, 16 ranks) steps whose B_a a thread has in registers
 
@@ -681,7 +692,8 @@ __host__ __device__ constexpr int lora_term_lists(int nt) { return nt <= 8 ? 2 :
 // The adapters of `nt` rows from t0 in groups of eight: two lists of pairs (slot;
 // group, and which of its rows use the slot) in group order, s_pair[0..] of the
 // even groups, s_pair[half..] of the odd ones, or of the only group's pairs in
-// turn, their lengths in s_count; one warp.  Their B_a for the features [n0, n0 + 128), contiguous, is on its way to L2.
+// turn, their lengths in s_count; one warp.  Their B_a for the features [n0, n0 +
+// 128), contiguous, is on its way to L2.
 DEVI void pair_adapters(const LoraParams& p, int t0, int nt, bool one_group, int n0, int half, int2* s_pair,
                         int* s_count) {
   const int lane = threadIdx.x & 31;
@@ -1027,7 +1039,10 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       const int at = (item >> 4) * 128 + q4;
 #pragma unroll 2
       for (int u = 0; u < split + lists; ++u) {  // the slices in order, then the adapters
-        const float* src = (u >= split ? s_terms + (u - split) * nt * 128 : u == rank ? part + t0 * 128 : recv + u * nt * 128) + at;
+        const float* src = u >= split   ? s_terms + (u - split) * nt * 128
+                           : u == rank ? part + t0 * 128
+                                       : recv + u * nt * 128;
+        src += at;
         const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + pair);
         lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
         hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
@@ -1071,7 +1086,8 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
   {
     std::lock_guard<std::mutex> lock(mu);
     if (!(ready >> dev & 1)) {
-      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM + BN * 512);  // (split 1: the most)
+      // (an unsplit K takes the most: the terms of BN rows)
+      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM + BN * 512);
       if (err != cudaSuccess) return err;
       ready |= uint64_t(1) << dev;
     }

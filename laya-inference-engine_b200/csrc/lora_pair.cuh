@@ -15,6 +15,15 @@
 // A block of 32 ranks of one of them is V's rows (TMA) against the B_a rows
 // (TMA); the builder warps clear the V rows of other adapters before the MMA.
 //
+// Bound by the tensor cores where there are tiles for every pair: 8,192 rows of K
+// 1,024 into 5,248 features 64 us (1.38 PFLOP/s; the library's plain product 66),
+// 77 with one adapter of rank 64 for all, 93 with 32 over 64 ragged requests: a
+// block of 32 ranks costs its hi and lo halves, as much as 64 of K, for all 256
+// rows, and such a tile has three adapters on average.  With few tiles by latency:
+// 1,536 rows of K 2,624 into 1,024 16.3 us, 8.8 of them the K blocks (L2 to shared
+// memory, 110 GB/s an SM), the rest the chain of the launches, the blocks of the
+// tile's five adapters (0.4 us each, from V's load to its MMAs) and the epilogue.
+//
 // Roles: warp 0 loads, warp 1 of the leader CTA issues the MMAs of both, warps
 // 2-3 build V tiles, warps 4-7 are the epilogue.  Every wait is bounded.
 #pragma once
@@ -52,7 +61,9 @@ struct PairCfg {
 DEVI void tmem_alloc2(uint32_t* slot) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
 }
-DEVI void tmem_relinquish2() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
+DEVI void tmem_relinquish2() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
 DEVI void tmem_dealloc2(uint32_t taddr) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
 }
