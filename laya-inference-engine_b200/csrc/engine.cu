@@ -1342,6 +1342,7 @@ int laya_b200_enable_adapters(laya_b200_engine* e, int slots, int max_rank) {
     uint8_t* base = e->weights->adapters;
     try {
       ck(cudaMemset(base, 0, off), "adapter slots");
+      ck(cudaStreamSynchronize(nullptr), "adapter slots");
       e->adapter_rank = rank;
       alloc_lora(e);
     } catch (...) {
@@ -1399,6 +1400,9 @@ int laya_b200_set_adapter(laya_b200_engine* e, int slot, const char* name, int r
     ck(cudaMemcpy(ad.a + (size_t)slot * R * K, pa.data(), pa.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
     ck(cudaMemcpy(ad.b + (size_t)slot * N * R, pb.data(), pb.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
     ck(cudaMemcpy(ad.scaling + slot, &scaling, 4, cudaMemcpyHostToDevice), "adapter upload");
+    // a copy from pageable memory may return before it has arrived, and the
+    // engines' streams do not wait for the default one
+    ck(cudaStreamSynchronize(nullptr), "adapter upload");
   });
 }
 

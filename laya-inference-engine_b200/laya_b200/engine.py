@@ -352,8 +352,11 @@ class B200Engine:
     def _adapter_slots(self, prepared, batch):
         slots = np.full(batch, -1, np.int32)
         for i, item in enumerate(prepared.items):
-            if item.get("adapter") is not None:
-                slots[i] = self.adapters[item["adapter"]]
+            name = item.get("adapter")
+            if name is not None:
+                if name not in self.adapters:  # unloaded since the request was checked
+                    raise ValueError(f"no adapter {name!r} is loaded")
+                slots[i] = self.adapters[name]
         return slots
 
     def _check_items(self, prepared, shape):

@@ -3,6 +3,7 @@ and the dispatcher that keeps every GPU's set, with fakes of the native engine."
 import queue
 import threading
 import time
+import types
 
 import numpy as np
 import pytest
@@ -268,3 +269,14 @@ def test_adapters_change_between_requests_only():
         d.unload_adapter("a")  # waits for the request, whose workers check that it is still loaded
         t.join()
         assert len(out) == 1 and all(d.healthy.values()) and e[0].adapters == {}
+
+
+def test_adapter_unloaded_between_check_and_run():
+    """The slots are looked up again when a lane takes the request."""
+    engine = B200Engine.__new__(B200Engine)
+    engine.adapters = {"a": 3}
+    prepared = types.SimpleNamespace(items=[{"adapter": "a"}, {}, {"adapter": None}])
+    assert engine._adapter_slots(prepared, 4).tolist() == [3, -1, -1, -1]
+    del engine.adapters["a"]
+    with pytest.raises(ValueError, match="no adapter 'a'"):
+        engine._adapter_slots(prepared, 4)
