@@ -106,23 +106,45 @@ at::Device device_of(std::initializer_list<const Tensor*> all) {
   return first.device();
 }
 
-// [first, last) byte address of what t covers (strides are not negative).
-void span_of(const Tensor& t, const char** lo, const char** hi) {
-  *lo = *hi = static_cast<const char*>(t.data_ptr());
-  if (t.numel() == 0) return;
-  int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  *hi = *lo + (last + 1) * (int64_t)t.element_size();
+// The bytes that t covers: [lo, hi), and, where its rows lie at one stride, that
+// stride and their width.
+struct Span {
+  const char *lo, *hi;
+  int64_t stride = 0, width = 0;
+};
+Span span_of(const Tensor& t) {
+  Span s{static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr())};
+  if (t.numel() == 0) return s;
+  const int64_t size = (int64_t)t.element_size(), dims = t.dim();
+  int64_t last = 0, outer = -1;
+  bool even = dims > 1 && (t.stride(dims - 1) == 1 || t.size(dims - 1) == 1);
+  for (int64_t d = dims - 1; d >= 0; --d) last += (t.size(d) - 1) * t.stride(d);
+  for (int64_t d = dims - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (outer < 0)
+      s.stride = t.stride(d) * size;
+    else
+      even = even && t.stride(d) == outer;
+    outer = t.stride(d) * t.size(d);
+  }
+  s.hi = s.lo + (last + 1) * size;
+  s.width = dims ? t.size(dims - 1) * size : size;
+  if (!even) s.stride = 0;
+  return s;
+}
+
+// Whether no byte is in both: apart, or columns of the same rows.
+bool apart(const Span& a, const Span& b) {
+  if (a.lo >= b.hi || b.lo >= a.hi) return true;
+  if (a.stride <= 0 || a.stride != b.stride) return false;
+  const int64_t at = (((b.lo - a.lo) % a.stride) + a.stride) % a.stride;  // where b's rows begin in a's
+  return at >= a.width && at + b.width <= a.stride;
 }
 
 void disjoint(const char* name, const Tensor& out, std::initializer_list<const Tensor*> others) {
-  const char *lo, *hi, *a, *b;
-  span_of(out, &lo, &hi);
+  const Span s = span_of(out);
   for (const Tensor* t : others)
-    if (t) {
-      span_of(*t, &a, &b);
-      if (a < hi && lo < b) refuse(std::string(name) + " overlaps another argument");
-    }
+    if (t && !apart(s, span_of(*t))) refuse(std::string(name) + " overlaps another argument");
 }
 
 void* ptr(const Tensor* t) { return t ? t->data_ptr() : nullptr; }

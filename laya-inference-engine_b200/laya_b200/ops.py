@@ -47,7 +47,9 @@ def rms_norm(x, weight=None, eps=1e-5, *, residual=None, out=None, dtype=None):
     ``x``: bf16 or fp32 ``[..., d]`` (d up to 16,384), rows at any stride.
     ``residual`` (bf16 or fp32, x's shape) is updated in place to h; the norm
     reads h before that rounding.  ``weight``: fp32 ``[d]`` or None.  Returns
-    ``out`` (``x`` itself is allowed), or a new tensor of ``dtype`` (x's)."""
+    ``out`` (``x`` itself is allowed), or a new tensor of ``dtype`` (x's).
+    ``residual`` and ``out`` may be other columns of x's rows; what shares bytes
+    with another argument is refused."""
     return _native.rms_norm(x, weight, eps, residual, out, dtype)
 
 

@@ -532,3 +532,34 @@ def test_first_call_inside_a_capture(which):
     done = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE, root, which], capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows, d", [(5, 64), (300, 72), (40, 1001)])
+def test_columns_of_one_buffer(rows, d):
+    """x, residual and output as columns of the same rows; what overlaps is refused."""
+    g = gen(80 + rows)
+    ld = 3 * d + 8 + (-3 * d) % 8
+    buffer = randn(g, rows, ld, dtype=BF16)
+    before = buffer.clone()
+    x, r, out = buffer[:, :d], buffer[:, d:2 * d], buffer[:, 2 * d + 1:3 * d + 1]
+    h, y = rms_reference(x, None, 1e-5, r)
+    ops.rms_norm(x, residual=r, out=out)
+    assert torch.equal(x, before[:, :d]) and torch.equal(r, h.float().to(BF16))
+    assert ((out.double() - y).abs() <= y_bound(y, BF16)).all()
+    assert torch.equal(buffer[:, 2 * d], before[:, 2 * d]) and torch.equal(buffer[:, 3 * d + 1:], before[:, 3 * d + 1:])
+    for lo in (1, d - 1, d + 1, 2 * d - 1):  # beside r's columns, partly over them
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.rms_norm(buffer[:, lo:lo + d], residual=r)
+    with pytest.raises(ValueError, match="overlaps"):  # other rows' strides
+        ops.rms_norm(buffer.view(-1)[:rows * d].view(rows, d), residual=r)
+    if d % 8:
+        return
+    n = 24
+    s = make(90 + rows, rows, d, n, 16, 3)
+    buffer[:, :d] = s["x"]
+    s["x"] = buffer[:, :d]
+    index = (torch.arange(rows, device=DEV) % 4 - 1).to(torch.int32)
+    ref = check_lora(s, index)
+    assert torch.equal(call(s, index, out=buffer[:, d:d + n]), ref) and torch.equal(buffer[:, :d], s["x"])
+    with pytest.raises(ValueError, match="overlaps"):
+        call(s, index, out=buffer[:, d - 1:d - 1 + n])
