@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(192)
       *failed = 0;
       fence_mbar_init();
       for (int k = 0; k < kShrinkFirst && k < nkb; ++k) load_rows(k, k);
+      for (int k = kShrinkFirst; k < nkb; ++k) tma_prefetch_2d(&xmap, (kb0 + k) * 64, row0);  // to L2, meanwhile
     }
     __syncwarp();
   } else if (warp == 5) {

@@ -79,6 +79,11 @@ DEVI bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, limit_ns));
 }
 
+// The block of a tensor map at (x, y) on its way to L2.
+DEVI void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+
 // One ring position: stage and the parity of its current use.
 template <int STAGES>
 struct Ring {

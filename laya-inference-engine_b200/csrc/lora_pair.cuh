@@ -217,9 +217,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     tmem_alloc2(tmem_slot);
     tmem_relinquish2();
   }
+  // (the barriers' initialisation is released by its own fence; the rest is this CTA's)
   tc_fence_before();
-  __syncwarp();
-  cluster_sync_all();
+  __syncthreads();
+  cluster_sync_relaxed();
   tc_fence_after();
   griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot;
@@ -549,7 +550,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   __syncwarp();
   griddep_wait();
   tc_fence_before();
-  cluster_sync_all();  // no CTA leaves while its partner may still signal it
+  // no CTA leaves while its partner may still signal it (with a release: the
+  // signals are to have arrived)
+  cluster_sync_all();
   if (warp == 2) tmem_dealloc2(tmem);
 }
 
