@@ -642,7 +642,7 @@ struct Fwd {
     lp.v = e->lora_v;
     lp.lists = e->lora_lists;
     lp.status = e->status_dev;
-    const int bnf = lora_pair_plan(w.kind, M, w.N, e->sm_count);
+    const int bnf = lora_pair_plan(w.kind, M, w.N, w.K, lp.rank, e->sm_count);
     int bn = 128, split = 1;
     if (!bnf) lora_few_plan(M, w.N, p.kblocks, e->sm_count, &bn, &split);
     p.tma_epilogue = bnf ? 1 : 0;
@@ -661,7 +661,8 @@ struct Fwd {
                                 : rows_map(&maps.out, out, M, epi == kEpiGeglu ? w.N / 2 : w.N, ldo, 2, 32));
     }
     if (!ok) fail("tensor map rejected for a %dx%d projection with adapters", M, w.N);
-    count(launch_lora_shrink(maps, lp, e->sm_count, bnf ? lora_pair_ctas(M, w.N, bnf, e->sm_count) : 0, st, pdl()),
+    count(launch_lora_shrink(maps, lp, e->sm_count, bnf ? lora_pair_ctas(M, w.N, bnf, e->sm_count) : 0,
+                             bnf ? lora_pair_us(w.kind, M, w.N, p.kblocks, bnf, e->sm_count) : 0.f, st, pdl()),
           "adapter shrink launch");
     count(bnf ? launch_lora_pairs(w.kind, maps, p, lp, bnf, st) : launch_lora_gemm(w.kind, maps, p, lp, bn, split, st),
           "adapter projection launch");

@@ -62,9 +62,10 @@ struct LoraMaps {
   CUtensorMap v;     // pairs: V as [rows][chunks * 64] bf16, 64 columns x 128 rows
   CUtensorMap out;   // pairs with p.tma_epilogue: output, 128 bytes of columns x 32 rows
 };
-// projection_ctas: CTAs of the projection behind it (launch_lora_pairs' grid), 0 for few rows.
+// projection_ctas, projection_us: the grid and the estimated time of the
+// launch_lora_pairs behind it, 0 for few rows.
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
-                               cudaStream_t stream, bool pdl);
+                               float projection_us, cudaStream_t stream, bool pdl);
 // Whether the shrink takes single dot products, without maps.rows and maps.a: up
 // to 64 rows, and 12M products: 16 rows, rank 64, K 2,624 8.9 us with the
 // projection (tiles on mma.sync 12.5); 64, 64, 2,624 14.1 (15.5); 64 rows of one
@@ -85,8 +86,10 @@ cudaError_t launch_lora_pairs(int kind, const LoraMaps& maps, const GemmParams& 
                               cudaStream_t stream);
 // CTAs of launch_lora_pairs for these sizes (at most the SMs).
 int lora_pair_ctas(int M, int N, int bnf, int sm_count);
+// Its time, roughly.
+float lora_pair_us(int kind, int M, int N, int kblocks, int bnf, int sm_count);
 // Features per tile of launch_lora_pairs, or 0 where launch_lora_gemm is to be used.
-int lora_pair_plan(int kind, int M, int N, int sm_count);
+int lora_pair_plan(int kind, int M, int N, int K, int rank, int sm_count);
 // Status of the launches that were given no status word; reading clears it.
 cudaError_t read_op_status(uint32_t* status);
 cudaError_t launch_rms_norm(const RmsNormParams& p, cudaStream_t stream, bool pdl);

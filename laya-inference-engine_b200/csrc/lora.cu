@@ -1155,8 +1155,53 @@ cudaError_t launch_shrink(const void* kern, int smem, int threads, dim3 grid, co
 
 }  // namespace
 
+namespace {
+
+// The tcgen05 shrink, one CTA per SM: K is split until they are in use (two K
+// blocks at least each), then the adapters, of which single rows of many requests
+// bring many.  On the SMs that the projection's CTAs leave, where it does not need
+// them all, both run side by side; on all of them it is done sooner, but the
+// projection waits (FP8, 2,048 rows of K 2,624 into 1,024 beside 64 pairs took 26.6
+// us, K not split; before them 18.6).  us: of both, roughly 3.5 us and 0.4 a K
+// block for the shrink.
+struct ShrinkPlan {
+  int room, split;  // CTAs per row tile and 64 ranks; K slices
+  float us;
+};
+ShrinkPlan shrink_plan(int rows, int rank, int in_features, int sm_count, int projection_ctas, float projection_us) {
+  const int tiles = (rows + kShrinkRows - 1) / kShrinkRows * ((rank + kShrinkRanks - 1) / kShrinkRanks);
+  const int kblocks = (in_features + 63) / 64, free_sms = sm_count - projection_ctas;
+  auto plan = [&](int room) {
+    int split = 1;
+    while (split < 8 && 4 * split <= kblocks && 2 * split <= room) split *= 2;
+    return ShrinkPlan{room, split, 3.5f + 0.4f * (float)kblocks / (float)split};
+  };
+  ShrinkPlan before = plan(std::max(1, sm_count / tiles));
+  before.us += projection_us;
+  if (free_sms < tiles) return before;
+  ShrinkPlan beside = plan(free_sms / tiles);
+  beside.us = std::max(beside.us, projection_us);
+  return beside.us <= before.us ? beside : before;
+}
+
+}  // namespace
+
+// The tiles with which both kernels are done sooner (bf16 takes 128 features where
+// 256 would leave pairs idle; FP8, 8,192 rows of K 2,624 into 1,024: 41.7 us with
+// 128, 37.2 with 256; K 1,024 into 5,248: 69.1, 68.1).
+int lora_pair_plan(int kind, int M, int N, int K, int rank, int sm_count) {
+  if (M <= kFewRows) return 0;
+  const int kblocks = (K + gemm_k_elems(kind) - 1) / gemm_k_elems(kind);
+  auto us = [&](int bnf) {
+    return shrink_plan(M, rank, K, sm_count, lora_pair_ctas(M, N, bnf, sm_count),
+                       lora_pair_us(kind, M, N, kblocks, bnf, sm_count))
+        .us;
+  };
+  return us(256) <= us(128) ? 256 : 128;
+}
+
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
-                               cudaStream_t stream, bool pdl) {
+                               float projection_us, cudaStream_t stream, bool pdl) {
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
       p.index_div < 1 || (!p.lists && lora_shrink_rows(p.rows) == kShrinkRows))
     return cudaErrorInvalidValue;
@@ -1192,16 +1237,10 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
     return wide ? launch_shrink((const void*)lora_shrink_few_kernel<true>, kWide, 160, grid, maps, p, stream, pdl)
                 : launch_shrink((const void*)lora_shrink_few_kernel<false>, kSlim, 160, grid, maps, p, stream, pdl);
   }
-  // One CTA per SM: K is split until they are in use (two K blocks at least
-  // each), then the adapters, of which single rows of many requests bring many.
   const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
-  // (the SMs that the projection's CTAs leave, where it does not need them all:
-  // both then run side by side)
-  const int free_sms = sm_count - projection_ctas;
-  const int room = std::max(1, (free_sms >= tiles * groups ? free_sms : sm_count) / (tiles * groups));
-  int split = 1;
-  while (split < 8 && 4 * split <= kblocks && 2 * split <= room) split *= 2;
-  const int slices = std::max(1, std::min(room / split, std::min(p.slots, std::min(p.rows, kShrinkRows))));
+  const ShrinkPlan plan = shrink_plan(p.rows, p.rank, p.in_features, sm_count, projection_ctas, projection_us);
+  const int split = plan.split;
+  const int slices = std::max(1, std::min(plan.room / split, std::min(p.slots, std::min(p.rows, kShrinkRows))));
   return launch_shrink((const void*)lora_shrink_kernel, kShrinkSmem, 192,
                        dim3(tiles, groups * slices, split), maps, p, stream, pdl);
 }

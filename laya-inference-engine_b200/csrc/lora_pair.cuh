@@ -54,7 +54,9 @@ struct PairCfg {
   static constexpr int K_ELEMS = KIND == kKindBf16 ? 64 : 128;
   // accumulators of one tile: the projection's, and for FP8 the adapters' own
   static constexpr int ACC_COLS = KIND == kKindFp8 ? 2 * BNF : BNF;
-  static_assert(2 * ACC_COLS <= 512, "two tiles in tensor memory");
+  // tiles in tensor memory: the epilogue of one runs under the MMAs of the next
+  // (FP8 with 256 features: one after the other)
+  static constexpr int TILES = 512 / ACC_COLS < 2 ? 1 : 2;
 };
 
 // ------------------------------------------------------------ pair primitives
@@ -177,8 +179,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   uint64_t* empty = full + ST;     // each CTA: the stage's MMAs are done
   uint64_t* vland = empty + ST;    // each CTA: its V rows have arrived
   uint64_t* vfull = vland + ST;    // leader: both CTAs' V tiles are built
-  uint64_t* acc_full = vfull + ST;     // each CTA: [2]
-  uint64_t* acc_empty = acc_full + 2;  // leader: [2]
+  constexpr int NT = C::TILES;
+  uint64_t* acc_full = vfull + ST;     // each CTA: [NT]
+  uint64_t* acc_empty = acc_full + 2;  // leader: [NT]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   uint32_t* failed = tmem_slot + 1;
   static_assert((4 * ST + 4) * 8 + 8 <= C::BAR_BYTES, "barrier block");
@@ -199,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       mbar_init(&vland[s], 1);
       mbar_init(&vfull[s], 4);  // two builder warps in each CTA
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < NT; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 8);  // four epilogue warps in each CTA
     }
@@ -283,13 +286,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     };
     // Both accumulators take their K blocks before the first adapter block has
     // to wait for the shrink.
-    const int t1 = pair + pairs < tiles ? pair + pairs : -1;
+    const int t1 = NT == 2 && pair + pairs < tiles ? pair + pairs : -1;
     k_blocks(pair);
     if (ok && t1 >= 0) k_blocks(t1);
     griddep_wait();
     if (ok) adapter_blocks(pair, head_of(pair % tiles_m));
     if (ok && t1 >= 0) adapter_blocks(t1, head_of(t1 % tiles_m));
-    for (int t = pair + 2 * pairs; t < tiles && ok; t += pairs) {
+    for (int t = pair + NT * pairs; t < tiles && ok; t += pairs) {
       const ListHead head = head_of(t % tiles_m);  // on its way during the K blocks
       k_blocks(t);
       if (ok) adapter_blocks(t, head);
@@ -313,8 +316,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     bool ok = true;
     // n: the tile's place among the pair's tiles
     auto k_blocks = [&](uint32_t n) {
-      const uint32_t acc = tmem + (n & 1) * 256;
-      if (n >= 2 && !(ok = warp_wait(&acc_empty[n & 1], ((n >> 1) - 1) & 1, limit))) return;
+      const uint32_t acc = tmem + n % NT * 256;
+      if (n >= NT && !(ok = warp_wait(&acc_empty[n % NT], (n / NT - 1) & 1, limit))) return;
       tc_fence_after();
       for (int kb = 0; kb < p.kblocks; ++kb, ring.next()) {
         const int s = ring.s;
@@ -335,7 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       }
     };
     auto adapter_blocks = [&](uint32_t n, int nb) {
-      const uint32_t acc2 = tmem + (n & 1) * 256 + (KIND == kKindFp8 ? BNF : 0);
+      const uint32_t acc2 = tmem + n % NT * 256 + (KIND == kKindFp8 ? BNF : 0);
       for (int b = 0; b < nb; ++b, ring.next()) {
         const int s = ring.s;
         if (!(ok = warp_wait(&full[s], ring.phase, limit)) || !(ok = warp_wait(&vfull[s], (vphase >> s) & 1, limit)))
@@ -354,17 +357,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         }
         __syncwarp();
       }
-      if (elect_one()) umma2_commit(&acc_full[n & 1]);
+      if (elect_one()) umma2_commit(&acc_full[n % NT]);
       __syncwarp();
     };
-    const int t1 = pair + pairs < tiles ? pair + pairs : -1;
+    const int t1 = NT == 2 && pair + pairs < tiles ? pair + pairs : -1;
     k_blocks(0);
     if (ok && t1 >= 0) k_blocks(1);
     griddep_wait();
     if (ok) adapter_blocks(0, blocks_of(pair % tiles_m));
     if (ok && t1 >= 0) adapter_blocks(1, blocks_of(t1 % tiles_m));
-    uint32_t n = 2;
-    for (int t = pair + 2 * pairs; t < tiles && ok; t += pairs, ++n) {
+    uint32_t n = NT;
+    for (int t = pair + NT * pairs; t < tiles && ok; t += pairs, ++n) {
       const int nb = blocks_of(t % tiles_m);  // on its way during the K blocks
       k_blocks(n);
       if (ok) adapter_blocks(n, nb);
@@ -382,8 +385,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       const int nb = head.count * lp.chunks;
       // the ring positions of the K blocks before: two tiles' before the first
       if (t == pair)
-        g = (pair + pairs < tiles ? 2 : 1) * p.kblocks;
-      else if (t >= pair + 2 * pairs)
+        g = (NT == 2 && pair + pairs < tiles ? 2 : 1) * p.kblocks;
+      else if (t >= pair + NT * pairs)
         g += p.kblocks;
       const int own0 = row_adapter(lp, m0 + r0), own1 = row_adapter(lp, m0 + r0 + 32);
       for (int b = 0; b < nb; ++b, ++g) {
@@ -416,7 +419,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     uint8_t* dst = staging + lq * 32 * 128;
     uint32_t n = 0;
     for (int t = pair; t < tiles; t += pairs, ++n) {
-      const int tm = t % tiles_m, tn = t / tiles_m, buf = n & 1;
+      const int tm = t % tiles_m, tn = t / tiles_m, buf = n % NT;
       const int mw = tm * 256 + (int)rank * 128 + lq * 32, m = mw + lane, n0 = tn * BNF;
       const bool second = KIND == kKindFp8 && blocks_of(tm) > 0;
       const float sa = KIND == kKindFp8 && m < p.M ? p.a_scale[m] : 1.f;
@@ -441,7 +444,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
           sn[4 * j] = b.x; sn[4 * j + 1] = b.y; sn[4 * j + 2] = b.z; sn[4 * j + 3] = b.w;
         }
       }
-      if (!warp_wait(&acc_full[buf], (n >> 1) & 1, limit)) {
+      if (!warp_wait(&acc_full[buf], n / NT & 1, limit)) {
         if (lane == 0) give_up(kStatusGemmDoneTimeout);
         break;
       }
@@ -607,17 +610,16 @@ cudaError_t launch_epilogue(const LoraMaps& maps, const GemmParams& p, const Lor
 
 }  // namespace
 
-int lora_pair_plan(int kind, int M, int N, int sm_count) {
-  if (M <= 64) return 0;
-  if (kind == kKindFp8) return 128;
-  // Waves of pairs times a tile's cost: a 128-feature tile takes about 0.7 of
-  // the time of a 256-feature one (shared-memory bandwidth).
-  const long long tm = (M + 255) / 256, pairs = sm_count / 2;
-  const long long wide = (tm * ((N + 255) / 256) + pairs - 1) / pairs;
-  const long long slim = (tm * ((N + 127) / 128) + pairs - 1) / pairs;
-  return 10 * wide <= 7 * slim ? 256 : 128;
+// Waves of tiles times a tile's cost.  A K block takes 0.31 us of a pair with 256
+// features and 0.215 with 128 (shared-memory and L2 bandwidth; FP8's hold twice
+// the columns), the epilogue 2.4 us, which only FP8 tiles of 256 features do not
+// hide under the next tile.
+float lora_pair_us(int kind, int M, int N, int kblocks, int bnf, int sm_count) {
+  const long long tiles = (long long)((M + 255) / 256) * ((N + bnf - 1) / bnf);
+  const float waves = (float)((tiles + sm_count / 2 - 1) / (sm_count / 2)), epilogue = 2.4f;
+  const float k = (float)kblocks * (bnf == 256 ? 0.31f : 0.215f);
+  return kind == kKindFp8 && bnf == 256 ? waves * (k + epilogue) : waves * k + epilogue;
 }
-
 int lora_pair_ctas(int M, int N, int bnf, int sm_count) {
   const long long tiles = (long long)((M + 255) / 256) * ((N + bnf - 1) / bnf);
   return (int)std::min<long long>(2 * tiles, sm_count);
@@ -628,6 +630,7 @@ cudaError_t launch_lora_pairs(int kind, const LoraMaps& maps, const GemmParams& 
   if (p.M < 1 || p.N < 1 || lp.rows != p.M || !lp.lists) return cudaErrorInvalidValue;
   if (kind == kKindBf16 && bnf == 256) return launch_epilogue<256, kKindBf16>(maps, p, lp, stream);
   if (kind == kKindBf16 && bnf == 128) return launch_epilogue<128, kKindBf16>(maps, p, lp, stream);
+  if (kind == kKindFp8 && bnf == 256) return launch_epilogue<256, kKindFp8>(maps, p, lp, stream);
   if (kind == kKindFp8 && bnf == 128) return launch_epilogue<128, kKindFp8>(maps, p, lp, stream);
   return cudaErrorInvalidValue;
 }

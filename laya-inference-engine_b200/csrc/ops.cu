@@ -82,7 +82,7 @@ bool lora_plan(const laya_b200_lora_args* a, int sm_count, LoraPlan* plan) {
   const int rows = a->rows > 0 ? a->rows : 1;
   auto align_up = [](size_t x) { return (x + 255) / 256 * 256; };
   plan->v_bytes = align_up((size_t)rows * ((a->rank + 31) / 32) * 128);
-  plan->bnf = lora_pair_plan(plan->kind, rows, a->out_features, sm_count);
+  plan->bnf = lora_pair_plan(plan->kind, rows, a->out_features, a->in_features, a->rank, sm_count);
   plan->list_bytes = plan->bnf ? align_up((size_t)((rows + 255) / 256) * kLoraListInts * sizeof(int)) : 0;
   if (!plan->bnf) lora_few_plan(rows, a->out_features, plan->kblocks, sm_count, &plan->bn, &plan->split);
   return true;
@@ -224,7 +224,8 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     if (plan.bnf) lp.lists = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.v_bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t err = launch_lora_shrink(
-        maps, lp, sms, plan.bnf ? lora_pair_ctas(M, N, plan.bnf, sms) : 0, st, true);
+        maps, lp, sms, plan.bnf ? lora_pair_ctas(M, N, plan.bnf, sms) : 0,
+        plan.bnf ? lora_pair_us(plan.kind, M, N, plan.kblocks, plan.bnf, sms) : 0.f, st, true);
     if (err != cudaSuccess) return reject("adapter shrink launch", err);
     err = plan.bnf ? launch_lora_pairs(plan.kind, maps, p, lp, plan.bnf, st)
                    : launch_lora_gemm(plan.kind, maps, p, lp, plan.bn, plan.split, st);
