@@ -640,15 +640,15 @@ struct Fwd {
     lp.b = ad.b;
     lp.scaling = ad.scaling;
     lp.v = e->lora_v;
-    lp.lists = e->lora_lists;
     lp.status = e->status_dev;
     const int bnf = lora_pair_plan(w.kind, M, w.N, w.K, lp.rank, e->sm_count);
+    if (bnf) lp.lists = e->lora_lists;
     int bn = 128, split = 1;
     if (!bnf) lora_few_plan(M, w.N, p.kblocks, e->sm_count, &bn, &split);
     p.tma_epilogue = bnf ? 1 : 0;
     const int wbox = bnf ? bnf / 2 : 128;
     LoraMaps maps{};
-    bool ok = (lora_shrink_by_row(M, lp.rank, w.K) ||
+    bool ok = ((!bnf && lora_shrink_by_row(M, lp.rank, w.K)) ||
                (rows_map(&maps.rows, x, M, w.K, w.K, 2, lora_shrink_rows(M)) &&
                 slots_map(&maps.a, ad.a, lp.slots, lp.rank, w.K, 64, lora_shrink_box(lp.rank),
                           CU_TENSOR_MAP_SWIZZLE_128B))) &&

@@ -66,17 +66,18 @@ struct LoraMaps {
 // launch_lora_pairs behind it, 0 for few rows.
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                float projection_us, cudaStream_t stream, bool pdl);
-// Whether the shrink takes single dot products, without maps.rows and maps.a: up
-// to 64 rows, and 12M products: 16 rows, rank 64, K 2,624 8.9 us with the
-// projection (tiles on mma.sync 12.5); 64, 64, 2,624 14.1 (15.5); 64 rows of one
-// adapter of rank 256, K 1,024, 17.8 (15.7).
+// Whether the shrink before launch_lora_gemm takes single dot products, without
+// maps.rows and maps.a; a dot product costs as much as 512 columns by itself.  With
+// the projection, dot products and tiles: 16 rows, rank 64, K 2,624 8.9 and 12.5 us;
+// 222, 40, 1,504 15.9 and 23.9; 64 rows of one adapter of rank 256, K 1,024, 17.8 and
+// 15.7; 829, 40, 264 17.7 and 14.1.
 inline bool lora_shrink_by_row(int rows, int rank, int in_features) {
-  return rows <= 64 && (long long)rows * rank * in_features <= 12 << 20;
+  return (long long)rows * rank * (in_features + 512) <= 20 << 20;
 }
 // Rows, and ranks of one adapter, in a CTA of the shrink.
 inline int lora_shrink_rows(int rows) { return rows <= 64 ? 64 : 128; }
 __host__ __device__ inline int lora_shrink_box(int rank) { return rank < 64 ? (rank + 15) / 16 * 16 : 64; }
-// The projection of up to 64 rows: row tile bn, K split over clusters.
+// The projection of few rows: row tiles of bn, K split over clusters.
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
                              int split, cudaStream_t stream);
 void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split);

@@ -4,10 +4,10 @@
 //   out[m] = X[m] W^T + s_a (X[m] A_a^T) B_a^T,   a = index[m / index_div]
 //
 // in two launches.  The shrink computes V[m] = s_a X[m] A_a^T, a few ranks per
-// row, in one of three kernels: lora_shrink_row_kernel (up to 64 rows, little
-// work: one dot product a warp), lora_shrink_few_kernel (up to 64 rows, mma.sync)
+// row, in one of three kernels: lora_shrink_row_kernel (little work: one dot
+// product a warp), lora_shrink_few_kernel (up to 64 rows, mma.sync)
 // and lora_shrink_kernel (tcgen05).  The projection takes the adapters in on the
-// way to its output, so that they cost no pass over it: lora_gemm_kernel (up to 64
+// way to its output, so that they cost no pass over it: lora_gemm_kernel (few
 // rows) adds their terms with its K slices, lora_pair_kernel lengthens its
 // reduction axis with the blocks of B_a.
 //
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(192)
     mbar_expect_tx(&full[s], kShrinkXBytes);
     tma_load_2d(sX + s * kShrinkXBytes, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
   };
-  const bool lists = row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1;  // this CTA writes the list of 256 rows
+  const bool lists = p.lists && row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1;  // this CTA writes the list of 256 rows
   int of_list[2] = {-1, -1};
   if (warp == 4) {
     if (elect_one()) {
@@ -653,8 +653,8 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
 }
 
 // ------------------------------------------------- projection for few rows
-// Up to 64 rows, bound by reading W and the adapters: the tile layout and
-// split-K of gemm.cu (weight rows on the TMEM lanes, rows of X as the MMA's N).
+// Few tiles, bound by reading W and the adapters: the tile layout and split-K of
+// gemm.cu (weight rows on the TMEM lanes, up to 64 rows of X as the MMA's N).
 // The adapters are not blocks of that reduction here.  A CTA stores BN / split
 // rows, and four warps compute those rows' adapter terms with mma.sync, in fp32,
 // while the K blocks and the exchange of the slices run: per group of eight rows
@@ -877,13 +877,14 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
   float* s_terms = reinterpret_cast<float*>(s_count + 4);  // [lists][BN / split][128] adapter terms
 
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int tile_n = blockIdx.x;
+  const int tile_n = blockIdx.x, m0 = blockIdx.y * BN;
+  const int rows = min(BN, p.M - m0);
   const int split = gridDim.z, rank = blockIdx.z;
   const int kb0 = (int)((long long)rank * p.kblocks / split);
   const int kb1 = (int)((long long)(rank + 1) * p.kblocks / split);
   const int nkb = kb1 - kb0;
   const int nt = BN / split, t0 = rank * nt;          // the tokens that this CTA stores,
-  const int stored = max(0, min(p.M - t0, nt));       // those that exist
+  const int stored = max(0, min(rows - t0, nt));       // those that exist
   const int lists = lora_term_lists(nt);
   uint32_t* status = p.status ? p.status : &g_op_status;
 
@@ -927,7 +928,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       if (elect_one()) {
         mbar_expect_tx(&full[s], C::STAGE_BYTES);
         tma_load_2d(sA + s * C::A_BYTES, &wmap, &full[s], (kb0 + i) * C::K_ELEMS, tile_n * 128, pol_w);
-        tma_load_2d(sB + s * C::B_BYTES, &xmap, &full[s], (kb0 + i) * C::K_ELEMS, 0, pol_x);
+        tma_load_2d(sB + s * C::B_BYTES, &xmap, &full[s], (kb0 + i) * C::K_ELEMS, m0, pol_x);
       }
       __syncwarp();
       issued = i + 1;
@@ -963,9 +964,9 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     const int bt = tid - 128, odd = (warp >> 1) & 1, half = (warp & 1) * 64;
     for (int i = bt; i < lists * nt * 32; i += 32 * kAdapterWarps)
       reinterpret_cast<float4*>(s_terms)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (warp == 4) pair_adapters(lp, t0, stored, lists == 2, tile_n * 128, BN / 2, s_pair, s_count);
+    if (warp == 4) pair_adapters(lp, m0 + t0, stored, lists == 2, tile_n * 128, BN / 2, s_pair, s_count);
     sync128();
-    AdapterTerms terms{lp, s_pair + odd * (BN / 2), s_count[odd], t0, stored};
+    AdapterTerms terms{lp, s_pair + odd * (BN / 2), s_count[odd], m0 + t0, stored};
     terms.start(tile_n * 128 + half);
     // (these warps have no part in the partial tile: they arrive at once, and wait
     // when they are done)
@@ -974,7 +975,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     terms.store_to(s_terms + odd * (lists - 1) * nt * 128 + half);
     if (split > 1) cluster_wait();
   } else if (KIND == kKindFp8) {
-    for (int i = tid - 64; i < BN; i += 64) s_scale[i] = i < p.M ? p.a_scale[i] : 0.f;
+    for (int i = tid - 64; i < BN; i += 64) s_scale[i] = i < rows ? p.a_scale[m0 + i] : 0.f;
   }
   __syncwarp();
 
@@ -993,13 +994,13 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     const float ws = KIND == kKindFp8 && tile_n * 128 + lr < p.N ? p.w_scale[tile_n * 128 + lr] : 1.f;
     constexpr int W = BN < 32 ? 16 : 32;
 #pragma unroll 1
-    for (int c = 0; c < BN && c < p.M; c += W) {
+    for (int c = 0; c < BN && c < rows; c += W) {
       uint32_t r[W];
       if constexpr (W == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
       tmem_wait_ld();
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        float v = __uint_as_float(r[j]);
+        float v = nkb > 0 ? __uint_as_float(r[j]) : 0.f;
         if (KIND == kKindFp8) v = (v * s_scale[c + j]) * ws;
         part[(c + j) * 128 + lr] = v;
       }
@@ -1013,7 +1014,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       if (warp == 0 && elect_one()) {
         mbar_expect_tx(sent, stored * (split - 1) * 512);
         for (int d = 1; d < split; ++d) {
-          const int to = (rank + d) % split, tokens = min(p.M - to * nt, nt);
+          const int to = (rank + d) % split, tokens = min(rows - to * nt, nt);
           if (tokens > 0)
             bulk_copy_to_peer(mapa_shared(smem_u32(recv + rank * nt * 128), to), part + to * nt * 128, tokens * 512,
                               mapa_shared(smem_u32(sent), to));
@@ -1033,7 +1034,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     const bool vec = p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
     for (int item = tid; item < stored * 16; item += C::THREADS) {
       const int q4 = rope ? ((item >> 3) & 1) * 64 + (item & 7) * 4 : (item & 15) * 4;
-      const int m = t0 + (item >> 4), n = tile_n * 128 + q4;
+      const int m = m0 + t0 + (item >> 4), n = tile_n * 128 + q4;
       EpiPre pre;
       if (!plain) pre = epi_prefetch<kKindBf16>(p, m, n, residual, rope);
       float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
@@ -1094,7 +1095,7 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N + 127) / 128, 1, split);
+  cfg.gridDim = dim3((p.N + 127) / 128, (p.M + BN - 1) / BN, split);
   cfg.blockDim = dim3(C::THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM + lora_term_lists(BN / split) * (BN / split) * 512;
   cfg.stream = stream;
@@ -1186,11 +1187,14 @@ ShrinkPlan shrink_plan(int rows, int rank, int in_features, int sm_count, int pr
 
 }  // namespace
 
-// The tiles with which both kernels are done sooner (bf16 takes 128 features where
+// Up to two tiles of 64 rows x 128 features for three SMs lora_gemm_kernel is done
+// sooner (331 rows of K 392 into 2,302 11.4 us, pairs 13.0; 102 rows with 25 adapters,
+// K 1,040 into 860, 10.6 and 26.5; but 605 rows of K 440 into 1,331 15.6 and 13.5).
+// Else the tiles with which both kernels are (bf16 takes 128 features where
 // 256 would leave pairs idle; FP8, 8,192 rows of K 2,624 into 1,024: 41.7 us with
 // 128, 37.2 with 256; K 1,024 into 5,248: 69.1, 68.1).
 int lora_pair_plan(int kind, int M, int N, int K, int rank, int sm_count) {
-  if (M <= kFewRows) return 0;
+  if (M <= kFewRows || 3ll * ((M + 63) / 64) * ((N + 127) / 128) <= 2 * sm_count) return 0;
   const int kblocks = (K + gemm_k_elems(kind) - 1) / gemm_k_elems(kind);
   auto us = [&](int bnf) {
     return shrink_plan(M, rank, K, sm_count, lora_pair_ctas(M, N, bnf, sm_count),
@@ -1203,7 +1207,7 @@ int lora_pair_plan(int kind, int M, int N, int K, int rank, int sm_count) {
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                float projection_us, cudaStream_t stream, bool pdl) {
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
-      p.index_div < 1 || (!p.lists && lora_shrink_rows(p.rows) == kShrinkRows))
+      p.index_div < 1)
     return cudaErrorInvalidValue;
   constexpr int kWide = FewShrinkCfg<true>::SMEM, kSlim = FewShrinkCfg<false>::SMEM;
   static std::mutex mu;
@@ -1223,10 +1227,10 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
     }
   }
   const int groups = (p.rank + kShrinkRanks - 1) / kShrinkRanks, kblocks = (p.in_features + 63) / 64;
+  if (!p.lists && lora_shrink_by_row(p.rows, p.rank, p.in_features))
+    return launch_shrink((const void*)lora_shrink_row_kernel, 0, 32 * kRowShrinkWarps,
+                         dim3(p.rank / kRowShrinkWarps, p.rows, 1), maps, p, stream, pdl);
   if (lora_shrink_rows(p.rows) == kFewRows) {
-    if (lora_shrink_by_row(p.rows, p.rank, p.in_features))
-      return launch_shrink((const void*)lora_shrink_row_kernel, 0, 32 * kRowShrinkWarps,
-                           dim3(p.rank / kRowShrinkWarps, p.rows, 1), maps, p, stream, pdl);
     // The adapters are spread first, then K, up to three CTAs per SM.
     const bool wide = p.rank > 32;
     const int per = (wide ? 64 : 32) / lora_shrink_box(p.rank), room = std::max(1, 3 * sm_count / groups);
@@ -1247,7 +1251,7 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
 
 cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int bn,
                              int split, cudaStream_t stream) {
-  if (p.M < 1 || p.M > bn || p.N < 1 || split < 1 || split > 8 || (split & (split - 1)) || split > p.kblocks ||
+  if (p.M < 1 || (p.M + bn - 1) / bn > 65535 || p.N < 1 || split < 1 || split > 8 || (split & (split - 1)) ||
       lp.rows != p.M || !lp.b)
     return cudaErrorInvalidValue;
   if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, maps, p, lp, split, stream);
@@ -1256,12 +1260,13 @@ cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p
 }
 
 // Row tile and K split of launch_lora_gemm.  Clusters of a power of two up to
-// about two CTAs per SM (a cluster of seven packs badly on the GPCs).
+// about two CTAs per SM (a cluster of seven packs badly on the GPCs); a CTA of more
+// than eight rows is split for its adapter terms too, where K blocks run out.
 void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split) {
   *bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-  const int tiles = (N + 127) / 128;
+  const long long tiles = (long long)((N + 127) / 128) * ((M + *bn - 1) / *bn);
   *split = 1;
-  while (*split < 8 && 2 * *split <= kblocks && 2 * *split * tiles <= 2 * sm_count) *split *= 2;
+  while (*split < 8 && (2 * *split <= kblocks || *bn / *split > 8) && 2 * *split * tiles <= 2 * sm_count) *split *= 2;
 }
 
 cudaError_t read_op_status(uint32_t* status) {

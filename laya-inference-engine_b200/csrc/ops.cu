@@ -183,7 +183,7 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     const int wbox = plan.bnf ? plan.bnf / 2 : 128;
     // rows of the output that take TMA stores
     const bool tma_out = plan.bnf && aligned(a->out, 16) && a->out_stride % 8 == 0;
-    bool ok = (lora_shrink_by_row(M, a->rank, K) ||
+    bool ok = ((!plan.bnf && lora_shrink_by_row(M, a->rank, K)) ||
                (rows_map(&maps.rows, a->x, M, K, a->x_stride, 2, lora_shrink_rows(M)) &&
                 slots_map(&maps.a, a->lora_a, a->slots, a->rank, K, 64, lora_shrink_box(a->rank),
                           CU_TENSOR_MAP_SWIZZLE_128B))) &&

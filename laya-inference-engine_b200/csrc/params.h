@@ -165,7 +165,7 @@ struct LoraParams {
   int out_features;
   const float* scaling;      // [slots] or null (1)
   __nv_bfloat16* v;          // [rows][chunks][64]
-  int* lists;                // [ceil(rows / 256)][kLoraListInts]; unused up to 64 rows
+  int* lists;                // [ceil(rows / 256)][kLoraListInts] for launch_lora_pairs, or null
   uint32_t* status;          // device-visible status word, or null
 };
 
