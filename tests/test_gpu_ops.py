@@ -563,3 +563,47 @@ def test_columns_of_one_buffer(rows, d):
     assert torch.equal(call(s, index, out=buffer[:, d:d + n]), ref) and torch.equal(buffer[:, :d], s["x"])
     with pytest.raises(ValueError, match="overlaps"):
         call(s, index, out=buffer[:, d - 1:d - 1 + n])
+
+
+@pytest.mark.parametrize("m, k, n, rank, slots", [(65, 64, 13000, 8, 3), (257, 512, 5000, 72, 40),
+                                                  (130, 256, 9001, 24, 130), (2000, 264, 1290, 40, 9),
+                                                  (6500, 2624, 1024, 16, 16)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_lora_linear_many_tiles(m, k, n, rank, slots, fp8):
+    """More tiles than the kernel for few of them takes: indices of every kind,
+    into strided outputs, and with values that are not finite."""
+    if fp8:
+        k = (k + 15) // 16 * 16
+    s = make(m * 5 + n, m, k, n, rank, slots, fp8, bias=n % 2 == 1)
+    index = runs(m, m, min(m, 30), slots)
+    ref = check_lora(s, index)
+    check_lora(s, (torch.arange(m, device=DEV) % slots).to(torch.int32))
+    check_lora(s, torch.full((m,), -1, dtype=torch.int32, device=DEV))
+    for pad in (0, 1, 5):
+        out = torch.full((m, n + 3 + pad), 5.0, dtype=BF16, device=DEV)
+        call(s, index, out=out[:, 2:2 + n])
+        assert torch.equal(out[:, 2:2 + n], ref) and (out[:, :2] == 5).all() and (out[:, 2 + n:] == 5).all()
+    index[::9] = slots - 1
+    ref = check_lora(s, index)
+    x, a = s["x"].clone(), s["a"].clone()
+    x[m // 2, 3], x[m - 1, k // 2] = float("nan"), float("inf")
+    got = call(dict(s, x=x), index)
+    others = torch.ones(m, dtype=torch.bool, device=DEV)
+    others[[m // 2, m - 1]] = False
+    assert torch.equal(got[others], ref[others])
+    a[slots - 1, 5, 9] = float("nan")
+    got = call(dict(s, a=a), index)
+    mine = index == slots - 1
+    assert torch.equal(got[~mine], ref[~mine]) and got[mine].isnan().all()
+    assert ops.op_status() == 0
+
+
+def test_first_and_last_rows_of_row_tiles():
+    """Rows behind the last one are left as they were."""
+    for m in (63, 64, 65, 127, 129, 192, 193, 255, 257):
+        s = make(m, m, 128, 40, 16, 5)
+        whole = torch.full((m + 70, 40), 3.0, dtype=BF16, device=DEV)
+        index = (torch.arange(m, device=DEV) % 6 - 1).to(torch.int32)
+        ref = check_lora(s, index)
+        call(s, index, out=whole[1:m + 1])
+        assert torch.equal(whole[1:m + 1], ref) and (whole[0] == 3).all() and (whole[m + 1:] == 3).all()
