@@ -668,7 +668,6 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
 // MMAs.)  Three stages: the shrink's CTAs then leave room for every CTA of this
 // kernel beside them (with four, the last ones started 4 us late).
 constexpr int kAdapterWarps = 4;
-constexpr int kAdapterAhead = 3;  // (adapter, 16 ranks) steps whose B_a a thread has in registers
 
 template <int BN, int KIND>
 struct LoraCfg {
@@ -723,63 +722,83 @@ DEVI void pair_adapters(const LoraParams& p, int t0, int nt, bool one_group, int
   }
 }
 
-// Four ranks, or zero.
-DEVI uint2 load_ranks_if(const __nv_bfloat16* p, bool in) {
-  uint2 v;
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %3, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n"
-      " @p ld.global.cg.v2.u32 {%0,%1}, [%2];\n}\n"
-      : "=r"(v.x), "=r"(v.y)
-      : "l"(p), "r"((int)in));
+// Four ranks (W = 1) or eight, or zero.
+template <int W>
+struct Ranks {
+  uint2 q[W];
+};
+template <int W>
+DEVI Ranks<W> load_ranks_if(const __nv_bfloat16* p, bool in) {
+  Ranks<W> v;
+  if constexpr (W == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %3, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n"
+        " @p ld.global.cg.v2.u32 {%0,%1}, [%2];\n}\n"
+        : "=r"(v.q[0].x), "=r"(v.q[0].y)
+        : "l"(p), "r"((int)in));
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n"
+        " mov.u32 %3, 0;\n @p ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+        : "=r"(v.q[0].x), "=r"(v.q[0].y), "=r"(v.q[W - 1].x), "=r"(v.q[W - 1].y)
+        : "l"(p), "r"((int)in));
   return v;
 }
-DEVI uint2 load_ranks(const __nv_bfloat16* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+template <int W>
+DEVI Ranks<W> load_ranks(const __nv_bfloat16* p) {
+  Ranks<W> v;
+  if constexpr (W == 1)
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.q[0].x), "=r"(v.q[0].y) : "l"(p));
+  else
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.q[0].x), "=r"(v.q[0].y), "=r"(v.q[W - 1].x), "=r"(v.q[W - 1].y)
+                 : "l"(p));
   return v;
 }
 // A warp's share of the adapter terms: 64 features from n0 (four m16 tiles) of a
-// list of pairs.  A step is 16 ranks of a pair; a lane holds four consecutive
-// ranks of a row of B_a and of V, which the instruction takes as two pairs: the
-// order of the ranks in its sum is free.  kAdapterAhead steps are in registers,
-// each one's place taken by its successor's loads at once, and the pair of the
-// next loads is read a step before them.  What a step has too many of (ranks,
-// features, steps behind the last) it loads from the nearest valid address and
-// multiplies with a zero V, or adds to a column that is not stored: one warp per
-// scheduler is bound by its instructions, and a predicate for each load doubled
-// them.
+// list of pairs.  A step is 16 W ranks of a pair; a lane holds 4 W consecutive
+// ranks of a row of B_a and of V, which an instruction takes four of as two pairs:
+// the order of the ranks in its sum is free.  AHEAD steps are in registers, each
+// one's place taken by its successor's loads at once, and the pair of the next
+// loads is read a step before them.  What a step has too many of (ranks, features,
+// steps behind the last) it loads from the nearest valid address and multiplies
+// with a zero V, or adds to a column that is not stored: one warp per scheduler is
+// bound by its instructions (0.3 us a step; a predicate for each load doubled them,
+// six steps ahead gained nothing).
+template <int W>
 struct AdapterTerms {
+  static constexpr int AHEAD = W == 1 ? 3 : 2;
   const LoraParams& p;
   const int2* s_pair;
   int pairs, t0, nt;
   int off[8];  // the lane's rows of B_a
-  uint2 b[kAdapterAhead][8], hi[kAdapterAhead], lo[kAdapterAhead];
-  int group[kAdapterAhead];  // -1 behind the last step
+  Ranks<W> b[AHEAD][8], hi[AHEAD], lo[AHEAD];
+  int group[AHEAD];  // -1 behind the last step
   int pair_b, k_b, pair_v, k_v;  // the next step to load
   int slot_b;
   int2 of_v;
 
   DEVI void next(int& pair, int& k) const {
-    k += 16;
+    k += 16 * W;
     const bool end = k >= p.rank;
     k = end ? 0 : k;
     pair += end;
   }
   DEVI void load_b(int u) {
-    const int k = min(k_b + 4 * (int)(threadIdx.x & 3), p.rank - 4);
+    const int k = min(k_b + 4 * W * (int)(threadIdx.x & 3), p.rank - 4 * W);
     const __nv_bfloat16* src = p.b + (size_t)(unsigned)slot_b * ((size_t)p.out_features * p.rank) + k;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[u][j] = load_ranks(src + off[j]);
+    for (int j = 0; j < 8; ++j) b[u][j] = load_ranks<W>(src + off[j]);
     next(pair_b, k_b);
     slot_b = s_pair[min(pair_b, pairs - 1)].x;
   }
   DEVI void load_v(int u) {
-    const int g = (threadIdx.x & 31) >> 2, k = k_v + 4 * (int)(threadIdx.x & 3);
+    const int g = (threadIdx.x & 31) >> 2, k = k_v + 4 * W * (int)(threadIdx.x & 3);
     const int to = of_v.y & 0xff, row = t0 + to * 8 + g;
     const bool in = pair_v < pairs && k < p.rank && (of_v.y >> (8 + g) & 1);
     const __nv_bfloat16* src = p.v + ((size_t)row * p.chunks + (k >> 5)) * 64 + (k & 31);
-    hi[u] = load_ranks_if(src, in);
-    lo[u] = load_ranks_if(src + 32, in);
+    hi[u] = load_ranks_if<W>(src, in);
+    lo[u] = load_ranks_if<W>(src + 32, in);
     group[u] = pair_v < pairs ? to : -1;
     next(pair_v, k_v);
     of_v = s_pair[min(pair_v, pairs - 1)];
@@ -794,7 +813,7 @@ struct AdapterTerms {
     of_v = s_pair[0];
     slot_b = of_v.x;
 #pragma unroll
-    for (int u = 0; u < kAdapterAhead; ++u) load_b(u);
+    for (int u = 0; u < AHEAD; ++u) load_b(u);
   }
   // out[row][128] = the terms (out: row t0, the warp's first feature)
   DEVI void store_to(float* out) {
@@ -802,11 +821,11 @@ struct AdapterTerms {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float acc[4][4] = {};
 #pragma unroll
-    for (int u = 0; u < kAdapterAhead; ++u) load_v(u);
+    for (int u = 0; u < AHEAD; ++u) load_v(u);
     int now = group[0];
     while (true) {
 #pragma unroll
-      for (int u = 0; u < kAdapterAhead; ++u) {
+      for (int u = 0; u < AHEAD; ++u) {
         if (group[u] != now) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -821,11 +840,14 @@ struct AdapterTerms {
           for (int m = 0; m < 4; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
         }
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const uint32_t a[4] = {b[u][m % 4 * 2].x, b[u][m % 4 * 2 + 1].x, b[u][m % 4 * 2].y, b[u][m % 4 * 2 + 1].y};
-          const uint2 v = m < 4 ? hi[u] : lo[u];
-          mma_bf16(acc[m % 4], a, v.x, v.y);
-        }
+        for (int w = 0; w < 2 * W; ++w)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const uint2 c = b[u][2 * m].q[w / 2], d = b[u][2 * m + 1].q[w / 2];
+            const uint2 v = w % 2 ? lo[u].q[w / 2] : hi[u].q[w / 2];
+            const uint32_t a[4] = {c.x, d.x, c.y, d.y};
+            mma_bf16(acc[m], a, v.x, v.y);
+          }
         load_b(u);
         load_v(u);
       }
@@ -854,7 +876,8 @@ DEVI void store_quad(const GemmParams& p, int m, int n, float4 v, bool vec) {
   }
 }
 
-template <int BN, int KIND>
+// W: AdapterTerms' (ranks above 16: 2).
+template <int BN, int KIND, int W>
 __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                      const GemmParams p, const LoraParams lp) {
@@ -966,7 +989,7 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
       reinterpret_cast<float4*>(s_terms)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (warp == 4) pair_adapters(lp, m0 + t0, stored, lists == 2, tile_n * 128, BN / 2, s_pair, s_count);
     sync128();
-    AdapterTerms terms{lp, s_pair + odd * (BN / 2), s_count[odd], m0 + t0, stored};
+    AdapterTerms<W> terms{lp, s_pair + odd * (BN / 2), s_count[odd], m0 + t0, stored};
     terms.start(tile_n * 128 + half);
     // (these warps have no part in the partial tile: they arrive at once, and wait
     // when they are done)
@@ -992,14 +1015,14 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
     const int lr = tid;  // weight row of the tile
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const float ws = KIND == kKindFp8 && tile_n * 128 + lr < p.N ? p.w_scale[tile_n * 128 + lr] : 1.f;
-    constexpr int W = BN < 32 ? 16 : 32;
+    constexpr int COLS = BN < 32 ? 16 : 32;
 #pragma unroll 1
-    for (int c = 0; c < BN && c < rows; c += W) {
-      uint32_t r[W];
-      if constexpr (W == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
+    for (int c = 0; c < BN && c < rows; c += COLS) {
+      uint32_t r[COLS];
+      if constexpr (COLS == 32) tmem_ld32(tmem + lane_addr + c, r); else tmem_ld16(tmem + lane_addr + c, r);
       tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
+      for (int j = 0; j < COLS; ++j) {
         float v = nkb > 0 ? __uint_as_float(r[j]) : 0.f;
         if (KIND == kKindFp8) v = (v * s_scale[c + j]) * ws;
         part[(c + j) * 128 + lr] = v;
@@ -1074,11 +1097,11 @@ __global__ void __launch_bounds__(LoraCfg<BN, KIND>::THREADS, 2)
 
 // ------------------------------------------------------------------ host side
 
-template <int BN, int KIND>
+template <int BN, int KIND, int W>
 cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int split,
                        cudaStream_t stream) {
   using C = LoraCfg<BN, KIND>;
-  auto kern = lora_gemm_kernel<BN, KIND>;
+  auto kern = lora_gemm_kernel<BN, KIND, W>;
   // Function attributes are per device: set them once for each device used.
   static std::mutex mu;
   static uint64_t ready = 0;
@@ -1114,13 +1137,13 @@ cudaError_t launch_one(const LoraMaps& maps, const GemmParams& p, const LoraPara
   return cudaLaunchKernelEx(&cfg, kern, maps.w, maps.x, p, lp);
 }
 
-template <int KIND>
+template <int KIND, int W>
 cudaError_t dispatch_bn(int bn, const LoraMaps& maps, const GemmParams& p, const LoraParams& lp, int split,
                         cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_one<16, KIND>(maps, p, lp, split, st);
-    case 32: return launch_one<32, KIND>(maps, p, lp, split, st);
-    case 64: return launch_one<64, KIND>(maps, p, lp, split, st);
+    case 16: return launch_one<16, KIND, W>(maps, p, lp, split, st);
+    case 32: return launch_one<32, KIND, W>(maps, p, lp, split, st);
+    case 64: return launch_one<64, KIND, W>(maps, p, lp, split, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -1254,8 +1277,13 @@ cudaError_t launch_lora_gemm(int kind, const LoraMaps& maps, const GemmParams& p
   if (p.M < 1 || (p.M + bn - 1) / bn > 65535 || p.N < 1 || split < 1 || split > 8 || (split & (split - 1)) ||
       lp.rows != p.M || !lp.b)
     return cudaErrorInvalidValue;
-  if (kind == kKindBf16) return dispatch_bn<kKindBf16>(bn, maps, p, lp, split, stream);
-  if (kind == kKindFp8) return dispatch_bn<kKindFp8>(bn, maps, p, lp, split, stream);
+  const bool wide = lp.rank > 16;
+  if (kind == kKindBf16)
+    return wide ? dispatch_bn<kKindBf16, 2>(bn, maps, p, lp, split, stream)
+                : dispatch_bn<kKindBf16, 1>(bn, maps, p, lp, split, stream);
+  if (kind == kKindFp8)
+    return wide ? dispatch_bn<kKindFp8, 2>(bn, maps, p, lp, split, stream)
+                : dispatch_bn<kKindFp8, 1>(bn, maps, p, lp, split, stream);
   return cudaErrorInvalidValue;
 }
 
