@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(192)
     mbar_expect_tx(&full[s], kShrinkXBytes);
     tma_load_2d(sX + s * kShrinkXBytes, &xmap, &full[s], (kb0 + k) * 64, row0, pol);
   };
-  const bool lists = p.lists && row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1;  // this CTA writes the list of 256 rows
+  // this CTA writes the list of 256 rows
+  const bool lists = p.lists && row0 % 256 == 0 && blockIdx.y == 0 && rank == split - 1;
   int of_list[2] = {-1, -1};
   if (warp == 4) {
     if (elect_one()) {
@@ -1189,21 +1190,28 @@ namespace {
 // us, K not split; before them 18.6).  us: of both, roughly 3.5 us and 0.4 a K
 // block for the shrink.
 struct ShrinkPlan {
-  int room, split;  // CTAs per row tile and 64 ranks; K slices
+  int split, slices;  // K slices; shares of a row tile's adapters
   float us;
 };
+// CTAs that run at a time in clusters of this size, one for an SM: the groups of SMs
+// that a cluster has to fit hold 15 clusters of eight and 33 of four on 148 SMs (a
+// few CTAs more ran as a second wave, 5 us after the first).
+int cluster_room(int sms, int size) { return size >= 8 ? sms * 120 / 148 : size == 4 ? sms * 132 / 148 : sms; }
+
 ShrinkPlan shrink_plan(int rows, int rank, int in_features, int sm_count, int projection_ctas, float projection_us) {
   const int tiles = (rows + kShrinkRows - 1) / kShrinkRows * ((rank + kShrinkRanks - 1) / kShrinkRanks);
   const int kblocks = (in_features + 63) / 64, free_sms = sm_count - projection_ctas;
-  auto plan = [&](int room) {
+  auto plan = [&](int sms) {
+    auto room = [&](int split) { return std::min(sms, cluster_room(sm_count, split)); };
     int split = 1;
-    while (split < 8 && 4 * split <= kblocks && 2 * split <= room) split *= 2;
-    return ShrinkPlan{room, split, 3.5f + 0.4f * (float)kblocks / (float)split};
+    while (split < 8 && 4 * split <= kblocks && 2 * split * tiles <= room(2 * split)) split *= 2;
+    const int slices = std::max(1, room(split) / (tiles * split));
+    return ShrinkPlan{split, slices, 3.5f + 0.4f * (float)kblocks / (float)split};
   };
-  ShrinkPlan before = plan(std::max(1, sm_count / tiles));
+  ShrinkPlan before = plan(sm_count);
   before.us += projection_us;
   if (free_sms < tiles) return before;
-  ShrinkPlan beside = plan(free_sms / tiles);
+  ShrinkPlan beside = plan(free_sms);
   beside.us = std::max(beside.us, projection_us);
   return beside.us <= before.us ? beside : before;
 }
@@ -1267,7 +1275,7 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
   const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
   const ShrinkPlan plan = shrink_plan(p.rows, p.rank, p.in_features, sm_count, projection_ctas, projection_us);
   const int split = plan.split;
-  const int slices = std::max(1, std::min(plan.room / split, std::min(p.slots, std::min(p.rows, kShrinkRows))));
+  const int slices = std::min(plan.slices, std::min(p.slots, std::min(p.rows, kShrinkRows)));
   return launch_shrink((const void*)lora_shrink_kernel, kShrinkSmem, 192,
                        dim3(tiles, groups * slices, split), maps, p, stream, pdl);
 }
@@ -1294,7 +1302,9 @@ void lora_few_plan(int M, int N, int kblocks, int sm_count, int* bn, int* split)
   *bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
   const long long tiles = (long long)((N + 127) / 128) * ((M + *bn - 1) / *bn);
   *split = 1;
-  while (*split < 8 && (2 * *split <= kblocks || *bn / *split > 8) && 2 * *split * tiles <= 2 * sm_count) *split *= 2;
+  while (*split < 8 && (2 * *split <= kblocks || *bn / *split > 8) &&
+         2 * *split * tiles <= 2 * cluster_room(sm_count, 2 * *split))
+    *split *= 2;
 }
 
 cudaError_t read_op_status(uint32_t* status) {
