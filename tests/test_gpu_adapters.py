@@ -120,7 +120,7 @@ def test_wide_network_takes_the_wide_tiles(precision):
     assert err <= TOL[precision], err
 
 
-def test_stages_with_adapters():
+def check_stages(shapes):
     """QKV with the rotary embedding, GEGLU and the residual sums of a one-layer
     network, each from the GPU's own stage before it, to a bf16 step."""
     cfg = LayaConfig(layers=1, hidden=256, heads=4, intermediate=384, vocab=1000, pad_token_id=999, max_len=512,
@@ -128,8 +128,8 @@ def test_stages_with_adapters():
     w = seeded_weights(cfg, seed=3)
     wf = {k: torch.from_numpy(v) for k, v in as_float32(w).items()}
     ad = {nm: (make_adapter(cfg, s, 12), 1.5) for s, nm in ((1, "a"), (2, "b"))}
-    for b, s in ((2, 192), (2, 32)):
-        items = synthetic_items([s, s], ["choice", "noul"], seed=11, vocab=cfg.vocab)
+    for b, s in shapes:
+        items = synthetic_items([s] * b, ["choice", "noul"] * (b // 2), seed=11, vocab=cfg.vocab)
         inp = pack(items, b, s, 4, cfg.pad_token_id)
         nf = NativeForward(0, cfg, w, "bf16", max_batch=b, max_options=4)
         try:
@@ -137,13 +137,13 @@ def test_stages_with_adapters():
             nf.set_adapter(0, *ad["a"])
             nf.set_adapter(1, *ad["b"])
             slot = nf.capture_adapters(b, s, 4, True)
-            nf.run(slot, inp, np.array([1, 0], np.int32))
+            nf.run(slot, inp, np.array([1, 0] * (b // 2), np.int32))
             T, d, inter = b * s, cfg.hidden, cfg.intermediate
             bits = {n: torch.from_numpy(bf16_bits_to_f32(nf.read_buffer(n, (T, c), np.uint16)))
                     for n, c in (("qkv", 3 * d), ("attn", d), ("g", inter))}
         finally:
             nf.close()
-        orc = AdaptedOracle(w, cfg, [ad["b"], ad["a"]])
+        orc = AdaptedOracle(w, cfg, [ad["b"], ad["a"]] * (b // 2))
         ids = torch.from_numpy(inp["input_ids"]).reshape(-1)
         h0 = O.layer_norm(wf["embed.tok"][ids], wf["embed.norm.w"], None, cfg.norm_eps)
         gcos, gsin = O.rope_tables(cfg.rope_theta_global, cfg.max_len, 64)
@@ -161,6 +161,15 @@ def test_stages_with_adapters():
             off = (bits[name] - ref).abs()
             assert (off <= steps * 2.0 ** -7 * ref.abs() + 2e-3).all(), (name, float(off.max()))
             assert float((off > 1e-6).float().mean()) < 0.05, name
+
+
+def test_stages_with_adapters():
+    check_stages(((2, 192), (2, 32)))
+
+
+def test_stages_with_adapters_over_many_tiles():
+    """The same on tiles of 256 rows, the residual projections among them."""
+    check_stages(((4, 512), (8, 512)))
 
 
 def test_no_adapter_in_an_adapted_batch():
