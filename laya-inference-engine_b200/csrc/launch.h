@@ -67,12 +67,13 @@ struct LoraMaps {
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                float projection_us, cudaStream_t stream, bool pdl);
 // Whether the shrink before launch_lora_gemm takes single dot products, without
-// maps.rows and maps.a; a dot product costs as much as 512 columns by itself.  With
-// the projection, dot products and tiles: 16 rows, rank 64, K 2,624 8.9 and 12.5 us;
-// 222, 40, 1,504 15.9 and 23.9; 64 rows of one adapter of rank 256, K 1,024, 17.8 and
-// 15.7; 829, 40, 264 17.7 and 14.1.
+// maps.rows and maps.a; a dot product costs as much as 512 columns by itself, and
+// tiles waste columns on small ranks.  With the projection, dot products and tiles:
+// 16 rows, rank 64, K 2,624 8.9 and 12.5 us; 222, 40, 1,504 15.9 and 23.9; 64 rows of
+// one adapter of rank 256, K 1,024, 17.8 and 15.7; 829, 40, 264 17.7 and 14.1; 64, 32,
+// 12,288 27.5 and 29.6; 64, 16, 40,000 87 and 69.
 inline bool lora_shrink_by_row(int rows, int rank, int in_features) {
-  return (long long)rows * rank * (in_features + 512) <= 20 << 20;
+  return (long long)rows * rank * (in_features + 512) <= (rank > 32 ? 20 : 32) << 20;
 }
 // Rows, and ranks of one adapter, in a CTA of the shrink.
 inline int lora_shrink_rows(int rows) { return rows <= 64 ? 64 : 128; }

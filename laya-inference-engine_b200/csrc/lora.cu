@@ -419,12 +419,9 @@ __global__ void __launch_bounds__(192)
 // us with the projection).
 constexpr int kFewRows = 64;
 
-// WIDE: one adapter of more than 32 ranks at a time; else adapters that
-// together have up to 32 columns, and a stage more in the same memory.
-template <bool WIDE>
 struct FewShrinkCfg {
-  static constexpr int COLS = WIDE ? 64 : 32;
-  static constexpr int STAGES = WIDE ? 3 : 4;
+  static constexpr int COLS = 64;  // of one adapter of more than 32 ranks, or of several at a time
+  static constexpr int STAGES = 3;
   static constexpr int X_BYTES = kFewRows * 128, A_BYTES = COLS * 128;
   static constexpr int PIPE_BYTES = STAGES * (X_BYTES + A_BYTES);
   static_assert(2 * kFewRows * (kShrinkRanks + 4) * 4 <= PIPE_BYTES, "the parts fit the pipeline's memory");
@@ -444,11 +441,10 @@ DEVI void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
                : "memory");
 }
 
-template <bool WIDE>
 __global__ void __launch_bounds__(160)
     lora_shrink_few_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
                        const LoraParams p) {
-  using C = FewShrinkCfg<WIDE>;
+  using C = FewShrinkCfg;
   constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1240,7 +1236,6 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
   if (p.rows < 1 || p.rank < 8 || p.rank % 8 || p.rank > kLoraMaxRank || p.in_features % 8 || p.slots < 1 ||
       p.index_div < 1)
     return cudaErrorInvalidValue;
-  constexpr int kWide = FewShrinkCfg<true>::SMEM, kSlim = FewShrinkCfg<false>::SMEM;
   static std::mutex mu;
   static uint64_t ready = 0;
   int dev = 0;
@@ -1251,8 +1246,7 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
     if (!(ready >> dev & 1)) {
       const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
       err = cudaFuncSetAttribute(lora_shrink_kernel, attr, kShrinkSmem);
-      if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_shrink_few_kernel<true>, attr, kWide);
-      if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_shrink_few_kernel<false>, attr, kSlim);
+      if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_shrink_few_kernel, attr, FewShrinkCfg::SMEM);
       if (err != cudaSuccess) return err;
       ready |= uint64_t(1) << dev;
     }
@@ -1263,14 +1257,12 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
                          dim3(p.rank / kRowShrinkWarps, p.rows, 1), maps, p, stream, pdl);
   if (lora_shrink_rows(p.rows) == kFewRows) {
     // The adapters are spread first, then K, up to three CTAs per SM.
-    const bool wide = p.rank > 32;
-    const int per = (wide ? 64 : 32) / lora_shrink_box(p.rank), room = std::max(1, 3 * sm_count / groups);
+    const int per = FewShrinkCfg::COLS / lora_shrink_box(p.rank), room = std::max(1, 3 * sm_count / groups);
     const int slices = std::min(room, (std::min(p.slots, p.rows) + per - 1) / per);
     int split = 1;
     while (split < 8 && 2 * split <= kblocks && 2 * split * slices <= room) split *= 2;
-    const dim3 grid(1, groups * slices, split);
-    return wide ? launch_shrink((const void*)lora_shrink_few_kernel<true>, kWide, 160, grid, maps, p, stream, pdl)
-                : launch_shrink((const void*)lora_shrink_few_kernel<false>, kSlim, 160, grid, maps, p, stream, pdl);
+    return launch_shrink((const void*)lora_shrink_few_kernel, FewShrinkCfg::SMEM, 160, dim3(1, groups * slices, split),
+                         maps, p, stream, pdl);
   }
   const int tiles = (p.rows + kShrinkRows - 1) / kShrinkRows;
   const ShrinkPlan plan = shrink_plan(p.rows, p.rank, p.in_features, sm_count, projection_ctas, projection_us);

@@ -607,3 +607,16 @@ def test_first_and_last_rows_of_row_tiles():
         ref = check_lora(s, index)
         call(s, index, out=whole[1:m + 1])
         assert torch.equal(whole[1:m + 1], ref) and (whole[0] == 3).all() and (whole[m + 1:] == 3).all()
+
+
+@pytest.mark.parametrize("m, k, n, rank, slots", [(64, 4096, 130, 128, 9), (37, 8192, 72, 200, 37), (64, 2048, 257, 256, 64),
+                                                  (64, 16384, 40, 24, 64), (33, 40000, 24, 16, 5), (64, 24000, 16, 32, 3),
+                                                  (64, 40968, 33, 8, 64), (64, 65536, 16, 8, 64),
+                                                  (61, 42000, 24, 24, 61)])
+def test_few_rows_of_much_work(m, k, n, rank, slots):
+    """V of up to 64 rows by tiles."""
+    s = make(m + rank, m, k, n, rank, slots, bias=n % 2 == 0)
+    check_lora(s, (torch.arange(m, device=DEV) % slots).to(torch.int32))
+    check_lora(s, runs(m + 3, m, 9, slots))
+    check_lora(s, torch.zeros(m, dtype=torch.int32, device=DEV))
+    assert ops.op_status() == 0
