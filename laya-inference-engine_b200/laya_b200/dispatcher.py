@@ -101,8 +101,9 @@ class B200Dispatcher:
         self.inflight = {d: None for d in self.devices}   # last future submitted to each worker
         self.lock = threading.Lock()
         self.adapters = {}      # name -> (adapter, scaling), what every healthy GPU has loaded
+        self._changes = threading.Lock()    # held to change what a GPU has loaded
         self._gate = threading.Condition()
-        self._running, self._changing = 0, False    # run_items calls; a change of the adapters
+        self._running, self._changing = 0, False    # run_items calls; a change of self.adapters
         self.closed = False
 
     def _run_batches(self, device, items, batches):
@@ -179,17 +180,17 @@ class B200Dispatcher:
 
     @contextmanager
     def _changing_adapters(self):
-        """No run_items in progress; those that follow wait."""
-        with self._gate:
-            self._gate.wait_for(lambda: not self._changing)
-            self._changing = True
-            self._gate.wait_for(lambda: self._running == 0)
-        try:
-            yield
-        finally:
+        """No run_items in progress and no other change; requests that follow wait."""
+        with self._changes:
             with self._gate:
-                self._changing = False
-                self._gate.notify_all()
+                self._changing = True
+                self._gate.wait_for(lambda: self._running == 0)
+            try:
+                yield
+            finally:
+                with self._gate:
+                    self._changing = False
+                    self._gate.notify_all()
 
     def load_adapter(self, name, adapter, scaling=1.0):
         """B200Engine.load_adapter on every healthy GPU, once no request is in
@@ -208,7 +209,7 @@ class B200Dispatcher:
                     self.engines[d].load_adapter(name, adapter, scaling)
                 except Exception:
                     for done in alive[:i + 1]:
-                        self._restore(done, name)
+                        self._restore_or_drop(done, name)
                     raise
             self.adapters[name] = (adapter, scaling)
 
@@ -223,17 +224,20 @@ class B200Dispatcher:
             with self.lock:
                 alive = [d for d in self.devices if self.healthy[d]]
             for d in alive:
-                self._restore(d, name)
+                self._restore_or_drop(d, name)
 
     def _restore(self, device, name):
-        """Bring one adapter of one GPU to what self.adapters holds; a GPU that
-        cannot leaves service."""
+        """Bring one adapter of one GPU to what self.adapters holds."""
         engine = self.engines[device]
+        if name in self.adapters:
+            engine.load_adapter(name, *self.adapters[name])
+        elif name in engine.adapters:
+            engine.unload_adapter(name)
+
+    def _restore_or_drop(self, device, name):
+        """_restore; a GPU that fails leaves service."""
         try:
-            if name in self.adapters:
-                engine.load_adapter(name, *self.adapters[name])
-            elif name in engine.adapters:
-                engine.unload_adapter(name)
+            self._restore(device, name)
         except Exception:
             with self.lock:
                 self.healthy[device] = False
@@ -258,18 +262,18 @@ class B200Dispatcher:
             self.inflight[d] = fut
             futures_wait([fut], timeout=timeout if timeout is not None else self.timeout)
             if fut.done() and fut.exception() is None:
-                names = {*self.adapters, *getattr(self.engines[d], "adapters", ())}
-                if not names:
+                # first what was loaded or unloaded while it was out.  No request runs
+                # on it meanwhile, so those in progress elsewhere need not end; but a
+                # change that began without it has to be over, and none may begin.
+                with self._changes:
+                    try:
+                        for name in {*self.adapters, *getattr(self.engines[d], "adapters", ())}:
+                            self._restore(d, name)
+                    except Exception:
+                        continue
                     with self.lock:
                         self.healthy[d] = True
-                else:  # first what was loaded or unloaded while it was out
-                    with self._changing_adapters():
-                        with self.lock:
-                            self.healthy[d] = True
-                        for name in names:
-                            self._restore(d, name)
-                if self.healthy[d]:
-                    back.append(d)
+                back.append(d)
         return back
 
     def close(self):
