@@ -248,10 +248,12 @@ class B200Dispatcher:
 
     def readmit(self, probe_items, timeout=None):
         """Probe every unhealthy GPU whose worker has returned with
-        `probe_items` (a small request) and mark it healthy again when the probe
-        succeeds.  Returns the devices put back in service."""
+        `probe_items` (a small request, run without adapters) and mark it healthy
+        again when the probe succeeds and it has every adapter that is loaded.
+        Returns the devices put back in service."""
         if self.closed:
             raise RuntimeError("Dispatcher is closed")
+        probe_items = [{**it, "adapter": None} if "adapter" in it else it for it in probe_items]
         back = []
         for d in self.devices:
             with self.lock:

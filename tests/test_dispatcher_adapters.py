@@ -128,3 +128,14 @@ def test_readmit_does_not_wait_for_requests():
         go.set()
         request.join()
         assert all(d.healthy.values())
+
+
+def test_probe_that_names_an_adapter():
+    """A probe runs without adapters: those of the GPU are restored after it."""
+    d, e = dispatcher()
+    with d:
+        drop_gpu_1(d, e)
+        d.load_adapter("a", PAIR)
+        probe = items("a")
+        assert d.readmit(probe) == [1] and e[1].adapters == {"a": 1.0}
+        assert probe == items("a")  # the caller's items are as they were
