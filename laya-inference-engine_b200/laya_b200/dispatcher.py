@@ -204,6 +204,8 @@ class B200Dispatcher:
         with self._changing_adapters():
             with self.lock:
                 alive = [d for d in self.devices if self.healthy[d]]
+            if not alive:
+                raise RuntimeError("no healthy GPU to load the adapter on")
             for i, d in enumerate(alive):
                 try:
                     self.engines[d].load_adapter(name, adapter, scaling)

@@ -139,3 +139,22 @@ def test_probe_that_names_an_adapter():
         probe = items("a")
         assert d.readmit(probe) == [1] and e[1].adapters == {"a": 1.0}
         assert probe == items("a")  # the caller's items are as they were
+
+
+def test_load_without_a_healthy_gpu():
+    """Nothing could check the adapter, and no GPU that it does not fit would return."""
+    d, e = dispatcher()
+    with d:
+        d.load_adapter("a", PAIR, 2.0)
+        e[0].fail = e[1].fail = True
+        with pytest.raises(RuntimeError, match="no healthy GPU"):
+            d.run_items(items(None, None, None, None))
+        with pytest.raises(RuntimeError, match="no healthy GPU"):
+            d.load_adapter("b", PAIR)
+        with pytest.raises(RuntimeError, match="no healthy GPU"):
+            d.load_adapter("a", PAIR, 3.0)
+        e[0].fail = e[1].fail = False
+        assert d.readmit(items(None)) == [0, 1]
+        assert e[0].adapters == e[1].adapters == {"a": 2.0}
+        d.unload_adapter("a")
+        assert e[0].adapters == e[1].adapters == {}
