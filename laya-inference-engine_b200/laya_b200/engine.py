@@ -461,9 +461,14 @@ class B200Engine:
                 for lane in held:
                     self._idle.put(lane)
 
-    def predict(self, state, questions):
+    def predict(self, state, questions, adapters=None):
+        """``adapters``: the adapter of every question by name, or a dict from
+        question id to name (questions that it leaves out, or gives None, run
+        on the shared weights alone)."""
         start = time.perf_counter()
         prepared = self.prepare(state, questions)
+        if adapters is not None:
+            prepared = _with_adapters(prepared, adapters)
         logits, act, metrics = self.run_prepared(prepared)
         result = format_response(prepared, logits, act, self.temperature, self.temperature_by_options)
         metrics["total_ms"] = (time.perf_counter() - start) * 1000
@@ -472,8 +477,8 @@ class B200Engine:
 
     system_one = predict
 
-    def warmup(self, state, questions):
-        return self.predict(state, questions)["engine"]
+    def warmup(self, state, questions, adapters=None):
+        return self.predict(state, questions, adapters)["engine"]
 
     def close(self):
         with self.lock:
@@ -507,6 +512,16 @@ def _load_weights(path):
     """Weights from an .npz holding the parameter table (bf16 as uint16)."""
     with np.load(path) as z:
         return {k: z[k] for k in z.files}
+
+
+def _with_adapters(prepared, adapters):
+    if not isinstance(adapters, dict):
+        adapters = dict.fromkeys(prepared.ids, adapters)
+    unknown = set(adapters) - set(prepared.ids)
+    if unknown:
+        raise ValueError(f"no question {sorted(map(str, unknown))} to give an adapter")
+    items = [{**item, "adapter": adapters.get(i)} for i, item in zip(prepared.ids, prepared.items)]
+    return PreparedRequest(prepared.ids, prepared.questions, items, prepared.input_tokens)
 
 
 def request_from_items(items):
