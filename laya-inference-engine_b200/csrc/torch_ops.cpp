@@ -167,7 +167,7 @@ void run_rms_norm(const Tensor& x, const Tensor* weight, double eps, const Tenso
   const Rows rx = rows_of("x", x, {kBF16, kF32});
   const int64_t d = rx.columns;
   if (d < 1 || d > 16384) refuse("x must have 1 to 16384 columns");
-  if (!(eps > 0) || std::isinf(eps)) refuse("eps must be positive and finite");
+  if (!((float)eps > 0) || std::isinf((float)eps)) refuse("eps must be positive and finite in fp32");
   if (weight) contiguous("weight", *weight, {d}, kF32);
   laya_b200_rms_norm_args a{};
   if (residual) {

@@ -13,9 +13,10 @@ the FP8 projection, its bf16 rows what the adapters read, and the projection's
 output the next norm's ``x``.  Every call runs on its tensors' device and that
 device's current stream, does not synchronise, allocates through torch's
 allocator only, and can be captured into a CUDA graph.  Arguments that an
-operator cannot take raise ValueError before anything is launched.  Inference
-only: no operator records a gradient, and tensors that require one are refused
-while gradients are enabled.  There is no CPU path.
+operator cannot take raise ValueError before anything is launched (sizes past the
+library's limits and operand rows off the 16-byte boundaries: RuntimeError, with
+its message).  Inference only: no operator records a gradient, and tensors that
+require one are refused while gradients are enabled.  There is no CPU path.
 """
 import ctypes
 import importlib.util
