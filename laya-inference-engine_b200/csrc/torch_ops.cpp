@@ -288,7 +288,7 @@ PyObject* py_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (slots < 1 || rank % 8 || rank < 8 || rank > 256)
     refuse("the adapters need at least one slot and a rank that is a multiple of 8 up to 256");
   if (per < 1) refuse("rows_per_index must be positive");
-  contiguous("index", index, {(rx.rows + per - 1) / per}, ScalarType::Int);
+  contiguous("index", index, {rx.rows / per + (rx.rows % per != 0)}, ScalarType::Int);
   if (scaling) contiguous("scaling", *scaling, {slots}, kF32);
   if (bias) contiguous("bias", *bias, {n}, kBF16);
   laya_b200_lora_args a{};
