@@ -147,6 +147,13 @@ void disjoint(const char* name, const Tensor& out, std::initializer_list<const T
     if (t && !apart(s, span_of(*t))) refuse(std::string(name) + " overlaps another argument");
 }
 
+// A tensor that a call has written: autograd refuses a graph that saved what it
+// held before, as it does after torch's in-place operators.  (Inference tensors have
+// no version.)
+void written(const Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void* ptr(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
 void check(const char* what, int status) {
@@ -202,6 +209,8 @@ void run_rms_norm(const Tensor& x, const Tensor* weight, double eps, const Tenso
   a.scale = static_cast<float*>(ptr(scale));
   const c10::cuda::CUDAGuard guard(dev);
   check("rms_norm", laya_b200_rms_norm(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  written(residual);
+  if (y_given) written(y);
 }
 
 // A new tensor beside x, without the dispatcher's microsecond (a tensor that is
@@ -337,6 +346,7 @@ PyObject* py_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::DataPtr work = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   check("lora_linear", laya_b200_lora_linear(&a, work.get(), bytes,
                                              c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  written(given);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
