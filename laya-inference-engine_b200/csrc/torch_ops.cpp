@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -91,16 +92,20 @@ void contiguous(const char* name, const Tensor& t, at::IntArrayRef shape, Scalar
     refuse(std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor of shape " + shape_of(shape));
 }
 
-// The CUDA device that all the tensors are on.
+// The CUDA device that all the tensors are on; tensors that a derivative would have
+// to be recorded for are refused.
 at::Device device_of(std::initializer_list<const Tensor*> all) {
   const Tensor& first = **all.begin();
   if (!first.is_cuda()) refuse("the operators run on CUDA tensors only");
-  bool grad = false;
+  bool grad = false, tangent = false;
   for (const Tensor* t : all)
     if (t) {
       if (t->device() != first.device()) refuse("tensors on " + t->device().str() + " and " + first.device().str());
       grad = grad || t->requires_grad();
+      tangent = tangent || t->_fw_grad(0).defined();
     }
+  if (tangent && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse("the operators compute no tangents; call them on fwAD.unpack_dual(x).primal");
   if (grad && c10::GradMode::is_enabled())
     refuse("the operators record no gradient; call them under torch.no_grad() or on detached tensors");
   return first.device();

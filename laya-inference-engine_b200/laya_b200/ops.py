@@ -15,9 +15,10 @@ device's current stream, does not synchronise, allocates through torch's
 allocator only, and can be captured into a CUDA graph.  Arguments that an
 operator cannot take raise ValueError before anything is launched (sizes past the
 library's limits and operand rows off the 16-byte boundaries: RuntimeError, with
-its message).  Inference only: no operator records a gradient, and tensors that
-require one are refused while gradients are enabled.  What a call writes in place
-counts as changed for autograd.  There is no CPU path.
+its message).  Inference only: no operator records a gradient or computes a
+tangent; tensors that require one are refused while gradients are enabled, and
+tensors that carry the other.  What a call writes in place counts as changed for
+autograd.  There is no CPU path.
 """
 import ctypes
 import importlib.util

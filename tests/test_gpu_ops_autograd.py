@@ -1,6 +1,8 @@
-"""The row operators beside autograd: what they write in place counts as changed."""
+"""The row operators beside autograd: what they write in place counts as changed,
+and tangents are refused as gradients are."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from laya_b200 import ops
 
@@ -78,3 +80,23 @@ def test_inference_tensors_are_written():
         ops.rms_norm(x, residual=h, out=y)
         ops.lora_linear(*lora_inputs(), out=torch.empty(4, 32, dtype=BF16, device=DEV))
     assert (h == 3).all()
+
+
+def test_tangents_are_refused():
+    x, r = torch.randn(4, 64, device=DEV), torch.randn(4, 64, device=DEV)
+    args, before = lora_inputs(), r.clone()
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(ValueError, match="tangent"):
+                    ops.rms_norm(dual)
+                with pytest.raises(ValueError, match="tangent"):
+                    ops.rms_norm_quant(x, residual=fwd.make_dual(r, torch.ones_like(r)))
+                for i in range(4):
+                    given = list(args)
+                    given[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises(ValueError, match="tangent"):
+                        ops.lora_linear(*given)
+        assert torch.equal(ops.rms_norm(fwd.unpack_dual(dual).primal), ops.rms_norm(x))
+    assert torch.equal(r, before) and ops.op_status() == 0
