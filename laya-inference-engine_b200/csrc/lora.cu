@@ -63,7 +63,7 @@ constexpr int kShrinkPipe = 4 * (kShrinkXBytes + kShrinkCols * 128);
 constexpr int kShrinkStages = 10;  // at most
 constexpr int kShrinkFirst = 4;  // row blocks requested before the adapters are known
 static_assert(2 * kShrinkRows * (kShrinkRanks + 4) * 4 <= kShrinkPipe, "the parts lie over the stages");
-constexpr int kListInts = 1536;  // write_list's memory
+constexpr int kListInts = 784;  // write_list's memory: the list, and number_adapters' for 256 rows
 constexpr int kShrinkSmem = kShrinkPipe + (3 * 128 + 264 + kListInts) * 4 + 256 + 1024;
 
 // The four warps that compute.
@@ -133,34 +133,15 @@ DEVI int number_adapters(int tid, const int (&own)[H], int (&ord)[H], int* s_lis
   return n;
 }
 
-// Writes the list of the 256 rows from row0 for the projection: count, adapters,
-// and each one's first and last row.  own: adapters of rows tid and 128 + tid;
-// 128 threads; `w`: 1536 ints of shared memory.
+// Writes the list of the 256 rows from row0 for the projection: count and adapters.
+// own: adapters of rows tid and 128 + tid; 128 threads; `w`: kListInts of shared memory.
 DEVI void write_list(const LoraParams& p, int row0, const int (&own)[2], int* w) {
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x;
   int ord[2] = {-1, -1};
-  int *s_list = w, *s_span = w + 256;
-  const int n = number_adapters<2>(tid, own, ord, s_list, w + 768, w + 1024, w + 1280);
-  for (int j = tid; j < n; j += 128) {
-    s_span[j] = 256;
-    s_span[256 + j] = -1;
-  }
-  sync128();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    // one lane of a warp's run speaks for it
-    const unsigned same = __match_any_sync(0xffffffffu, ord[h]);
-    if (ord[h] >= 0 && __ffs(same) - 1 == lane) {
-      atomicMin(&s_span[ord[h]], h * 128 + tid);
-      atomicMax(&s_span[256 + ord[h]], h * 128 + tid - lane + 31 - __clz(same));
-    }
-  }
-  sync128();
+  int* s_list = w;
+  const int n = number_adapters<2>(tid, own, ord, s_list, w + 256, w + 512, w + 768);
   int* out = p.lists + (size_t)(row0 / 256) * kLoraListInts;
-  for (int j = tid; j < n; j += 128) {
-    out[kLoraListSlots + j] = s_list[j];
-    out[kLoraListSpans + j] = s_span[j] | s_span[256 + j] << 16;
-  }
+  for (int j = tid; j < n; j += 128) out[kLoraListSlots + j] = s_list[j];
   if (tid == 0) out[0] = n;
 }
 

@@ -148,8 +148,8 @@ struct QuantParams {
 // Low-rank adapters beside a projection (lora.cu).  V[m] holds the adapter's
 // inner row s_a x[m] A_a^T as chunks of 32 ranks, each 128 bytes [hi 32 | lo 32].
 constexpr int kLoraMaxRank = 256;
-// Adapters that 256 rows use: their count, [256] adapters, [256] first row | last row << 16.
-constexpr int kLoraListSlots = 4, kLoraListSpans = 260, kLoraListInts = 516;
+// Adapters that 256 rows use: their count, and (on a 16-byte boundary) [256] adapters.
+constexpr int kLoraListSlots = 4, kLoraListInts = 260;
 struct LoraParams {
   int rows;
   int in_features;           // multiple of 8
