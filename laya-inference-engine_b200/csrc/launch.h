@@ -49,10 +49,11 @@ cudaError_t launch_gather_rows(float* dst, const float* src, const int* map, int
                                bool pdl);
 cudaError_t launch_tail(const TailParams& p, int batch, cudaStream_t stream, bool pdl);
 cudaError_t launch_token_gather(const TokenGatherParams& p, cudaStream_t stream, bool pdl);
-// Adapters beside a projection (lora.cu): the shrink V = s x A^T; for more than
-// 64 rows it also lists the adapters of every 256; then the projection that adds V B^T;
-// launched one behind the other on one stream.  Tensor maps (128-byte swizzle
-// and boxes of 128 bytes of K unless said otherwise):
+// Adapters beside a projection (lora.cu): the shrink V = s x A^T, which before
+// launch_lora_pairs (p.lists given: lora_pair_plan is not 0) also lists the adapters
+// of every 256 rows; then the projection that adds V B^T; launched one behind the
+// other on one stream.  Tensor maps (128-byte swizzle and boxes of 128 bytes of K
+// unless said otherwise):
 struct LoraMaps {
   CUtensorMap rows;  // X as bf16, lora_shrink_rows(rows) rows
   CUtensorMap a;     // A [slots][rank][K] bf16, lora_shrink_box(rank) ranks of one slot
@@ -63,7 +64,7 @@ struct LoraMaps {
   CUtensorMap out;   // pairs with p.tma_epilogue: output, 128 bytes of columns x 32 rows
 };
 // projection_ctas, projection_us: the grid and the estimated time of the
-// launch_lora_pairs behind it, 0 for few rows.
+// launch_lora_pairs behind it, 0 before launch_lora_gemm.
 cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm_count, int projection_ctas,
                                float projection_us, cudaStream_t stream, bool pdl);
 // Whether the shrink before launch_lora_gemm takes single dot products, without

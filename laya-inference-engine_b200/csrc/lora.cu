@@ -742,7 +742,9 @@ DEVI Ranks<W> load_ranks(const __nv_bfloat16* p) {
 // steps behind the last) it loads from the nearest valid address and multiplies
 // with a zero V, or adds to a column that is not stored: one warp per scheduler is
 // bound by its instructions (0.3 us a step; a predicate for each load doubled them,
-// six steps ahead gained nothing).
+// six steps ahead gained nothing).  With W = 2 the two steps of B_a take 64 of the
+// 128 registers that two CTAs an SM leave a thread, and 88 bytes of a thread spill
+// (W = 1: none).
 template <int W>
 struct AdapterTerms {
   static constexpr int AHEAD = W == 1 ? 3 : 2;

@@ -7,9 +7,12 @@
 // memory per 256 x 256 x 16 step where a lone CTA's 128 x 128 tile reads twice
 // that per unit of work; shared-memory bandwidth is what holds the 128 x 128
 // tiles of gemm.cu at half of the tensor cores' rate.  Rows sit on the TMEM
-// lanes, so an epilogue thread owns one row of the output and stores whole
-// 32-byte sectors of it straight from registers; the tensor memory holds two
-// accumulators, and the epilogue of one tile runs under the MMAs of the next.
+// lanes, so an epilogue thread owns one row of the output; it writes to its warp's
+// swizzled block of 32 rows x 128 bytes, which a TMA store (residual: a TMA
+// addition) or, where the output's rows take no TMA, the lanes along the rows bring
+// to memory.  The tensor memory holds two accumulators (FP8 tiles of 256 features:
+// one and the adapters' own), and the epilogue of one tile then runs under the MMAs
+// of the next.
 //
 // Adapters: the shrink lists, for each 256-row tile, the adapters its rows use.
 // A block of 32 ranks of one of them is V's rows (TMA) against the B_a rows
@@ -213,9 +216,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     prefetch_tensormap(&bmap);
     prefetch_tensormap(&vmap);
   }
-  // All of the tensor memory: the kernels before this one are complete (the
-  // shrink waited for them and uses none), and the next one is released only
-  // after the allocation, so neither can hold what the other waits for.
+  // All of the tensor memory.  The shrink before may still hold its 256 columns: its
+  // CTAs have allocated before they release this kernel and free without waiting for
+  // it, so this allocation at most waits for them (their shared memory does not fit
+  // beside this kernel's on one SM either).  What came before the shrink is complete.
+  // The next kernel is released only after this allocation.
   if (warp == 2) {
     tmem_alloc2(tmem_slot);
     tmem_relinquish2();
