@@ -69,10 +69,11 @@ cudaError_t launch_lora_shrink(const LoraMaps& maps, const LoraParams& p, int sm
                                float projection_us, cudaStream_t stream, bool pdl);
 // Whether the shrink before launch_lora_gemm takes single dot products, without
 // maps.rows and maps.a; a dot product costs as much as 512 columns by itself, and
-// tiles waste columns on small ranks.  With the projection, dot products and tiles:
-// 16 rows, rank 64, K 2,624 8.9 and 12.5 us; 222, 40, 1,504 15.9 and 23.9; 64 rows of
-// one adapter of rank 256, K 1,024, 17.8 and 15.7; 829, 40, 264 17.7 and 14.1; 64, 32,
-// 12,288 27.5 and 29.6; 64, 16, 40,000 87 and 69.
+// tiles waste columns on small ranks.  With the projection into 512 features, dot
+// products and tiles: 16 rows, rank 64, K 2,624 7.8 and 12.4 us; 222, 40, 1,504 12.4
+// and 14.9; 829, 40, 264 19.7 and 16.8; 64, 32, 12,288 18.4 and 32.5; 64, 16, 40,000
+// 74 and 59; 64 rows of rank 256, K 1,024: one adapter 15.2 and 13.1, 64 of them 29
+// and 40 (the adapters that the rows name are not known here).
 inline bool lora_shrink_by_row(int rows, int rank, int in_features) {
   return (long long)rows * rank * (in_features + 512) <= (rank > 32 ? 20 : 32) << 20;
 }

@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(192)
 // The same for up to 64 rows, which may each bring an adapter of their own:
 // CTAs of 64 rows on mma.sync, whose operands TMA stages, without tensor memory
 // and in little shared memory, so that several share an SM and the projection's
-// CTAs start beside them (64 rows of one adapter of rank 256, K and N 1,024: 15.7
+// CTAs start beside them (64 rows of one adapter of rank 256, K and N 1,024: 13.5
 // us with the projection).
 constexpr int kFewRows = 64;
 
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(32 * kRowShrinkWarps) lora_shrink_row_kernel(c
 // and adapter that they use, 16 ranks a step, the other rows' V zero.  B_a goes
 // from memory to registers, the first of it before V is there, and the terms wait
 // for no stage.  Measured, 64 rows with 64 adapters of rank 16 into 5,248 features:
-// 10.7 us, 8.5 with one adapter, 8.2 with none (the bytes take 3.5): the two
+// 10.9 us, 8.9 with one adapter, 8.6 with none (the bytes take 3.5): the two
 // launches' chain, then 0.3 us a step, which is the loads' latency over the three
 // steps that registers hold.  (As K blocks of the tcgen05 pipeline, V tiles built
 // in shared memory, 17.7 us: a block took 0.5 us from its stage's release to its

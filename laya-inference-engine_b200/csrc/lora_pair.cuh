@@ -18,14 +18,16 @@
 // A block of 32 ranks of one of them is V's rows (TMA) against the B_a rows
 // (TMA); the builder warps clear the V rows of other adapters before the MMA.
 //
-// Bound by the tensor cores where there are tiles for every pair: 8,192 rows of K
-// 1,024 into 5,248 features 64 us (1.38 PFLOP/s; the library's plain product 66),
-// 77 with one adapter of rank 64 for all, 93 with 32 over 64 ragged requests: a
-// block of 32 ranks costs its hi and lo halves, as much as 64 of K, for all 256
-// rows, and such a tile has three adapters on average.  With few tiles by latency:
-// 1,536 rows of K 2,624 into 1,024 16.3 us, 8.8 of them the K blocks (L2 to shared
-// memory, 110 GB/s an SM), the rest the chain of the launches, the blocks of the
-// tile's five adapters (0.4 us each, from V's load to its MMAs) and the epilogue.
+// Bound by the tensor cores where there are tiles for every pair, and by the clock
+// that the power limit leaves them: 8,192 rows of K 1,024 into 5,248 features 66 us
+// (1.33 PFLOP/s; the library's plain product 67) in a short burst of replays and 77
+// (79) in a second of them at about 1.5 GHz, 76 and 88 with one adapter of rank 64
+// for all, 93 and 108 to 112 with 32 over 64 ragged requests: a block of 32 ranks
+// costs its hi and lo halves, as much as 64 of K, for all 256 rows, and such a tile
+// has three adapters on average.  With few tiles by latency: 1,536 rows of K 2,624
+// into 1,024 15.8 us, 8.8 of them the K blocks (L2 to shared memory, 110 GB/s an SM),
+// the rest the chain of the launches, the blocks of the tile's five adapters (0.4 us
+// each, from V's load to its MMAs) and the epilogue.
 //
 // Roles: warp 0 loads, warp 1 of the leader CTA issues the MMAs of both, warps
 // 2-3 build V tiles, warps 4-7 are the epilogue.  Every wait is bounded.

@@ -10,11 +10,13 @@
 // norm reads the unrounded sum and the quantiser the unrounded y, so each
 // output is rounded once.  One pass over memory, which is what bounds it: a row's
 // elements stay in the registers of a warp (short rows, shuffles only) or of a CTA.
-// Measured against bytes / 6,556 GB/s (a copy's rate): 32,768 rows of 1,024 with an
-// fp32 residual and codes 58.1 us (97 %), 16,384 of 4,096 in bf16 82.3 (99 %), 4,000
-// of 8,191 71 (84 %), 14,427 of 435 15.2 (76 %).  Rows with little to load for what
-// they compute are bound by the chain load - sum - weight - maximum - store of the
-// rows in flight: bf16 rows without a residual 71 to 78 %, with codes 34 %.
+// Measured in replayed graphs against bytes / 6,556 GB/s (a copy's rate): 32,768 rows
+// of 1,024 with an fp32 residual and codes 61 us (92 %; 58 in a short burst, before
+// the power limit lowers the clock), 16,384 of 4,096 in bf16 83 to 86 (95 to 99 %),
+// 4,000 of 8,191 71 (84 %), 14,427 of 435 14.9 (77 %).  Rows with little to load for
+// what they compute are bound by the chain load - sum - weight - maximum - store of
+// the rows in flight: 32,768 bf16 rows of 1,024 without a residual 26 us (78 %), to
+// codes alone 35 (44 %).  The comparisons of two forms below are of short bursts.
 #include "common.cuh"
 #include "params.h"
 #include "launch.h"
