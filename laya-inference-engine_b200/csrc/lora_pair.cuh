@@ -138,7 +138,7 @@ DEVI void tma_add_2d(const CUtensorMap* map, const void* src, int x, int y) {
 
 // A warp's block of 32 rows x 64 bf16 columns (128-byte swizzle) to rows m0..,
 // columns n.. where the output's rows do not take TMA stores (unaligned rows or
-// strides): its lanes store along the rows.
+// strides, widths that end inside 16 bytes): its lanes store along the rows.
 DEVI void store_block(const GemmParams& p, int m0, int n, const uint8_t* block) {
   const int lane = threadIdx.x & 31, rows = min(32, p.M - m0);
   const bool in0 = n + lane < p.N, in1 = n + lane + 32 < p.N;

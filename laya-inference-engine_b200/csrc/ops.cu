@@ -181,8 +181,9 @@ extern "C" int laya_b200_lora_linear(const laya_b200_lora_args* a, void* workspa
     const void* operand = a->codes ? a->codes : a->x;
     const long long ldo = a->codes ? a->codes_stride : a->x_stride;
     const int wbox = plan.bnf ? plan.bnf / 2 : 128;
-    // rows of the output that take TMA stores
-    const bool tma_out = plan.bnf && aligned(a->out, 16) && a->out_stride % 8 == 0;
+    // rows of the output that take TMA stores, which write whole 16 bytes: those of a
+    // width that ends inside one would go over the columns behind it
+    const bool tma_out = plan.bnf && aligned(a->out, 16) && a->out_stride % 8 == 0 && N % 8 == 0;
     bool ok = ((!plan.bnf && lora_shrink_by_row(M, a->rank, K)) ||
                (rows_map(&maps.rows, a->x, M, K, a->x_stride, 2, lora_shrink_rows(M)) &&
                 slots_map(&maps.a, a->lora_a, a->slots, a->rank, K, 64, lora_shrink_box(a->rank),
