@@ -1342,8 +1342,8 @@ int laya_b200_enable_adapters(laya_b200_engine* e, int slots, int max_rank) {
     ck(cudaMalloc(&e->weights->adapters, off), "adapter slots");
     uint8_t* base = e->weights->adapters;
     try {
-      ck(cudaMemset(base, 0, off), "adapter slots");
-      ck(cudaStreamSynchronize(nullptr), "adapter slots");
+      ck(cudaMemsetAsync(base, 0, off, e->stream), "adapter slots");
+      ck(cudaStreamSynchronize(e->stream), "adapter slots");
       e->adapter_rank = rank;
       alloc_lora(e);
     } catch (...) {
@@ -1398,12 +1398,15 @@ int laya_b200_set_adapter(laya_b200_engine* e, int slot, const char* name, int r
       memcpy(pb.data() + (size_t)r * R, hb + (size_t)src * rank, (size_t)rank * 2);
     }
     const AdapterSet& ad = e->adapters[index];
-    ck(cudaMemcpy(ad.a + (size_t)slot * R * K, pa.data(), pa.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
-    ck(cudaMemcpy(ad.b + (size_t)slot * N * R, pb.data(), pb.size() * 2, cudaMemcpyHostToDevice), "adapter upload");
-    ck(cudaMemcpy(ad.scaling + slot, &scaling, 4, cudaMemcpyHostToDevice), "adapter upload");
-    // a copy from pageable memory may return before it has arrived, and the
-    // engines' streams do not wait for the default one
-    ck(cudaStreamSynchronize(nullptr), "adapter upload");
+    auto upload = [&](void* dst, const void* src, size_t bytes) {
+      ck(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, e->stream), "adapter upload");
+    };
+    upload(ad.a + (size_t)slot * R * K, pa.data(), pa.size() * 2);
+    upload(ad.b + (size_t)slot * N * R, pb.data(), pb.size() * 2);
+    upload(ad.scaling + slot, &scaling, 4);
+    // the lanes' streams do not wait for this one; nor does this wait for the whole
+    // device, which another engine's capture forbids
+    ck(cudaStreamSynchronize(e->stream), "adapter upload");
   });
 }
 
@@ -1416,11 +1419,11 @@ int laya_b200_clear_adapter(laya_b200_engine* e, int slot) {
         const ParamInfo& pi = e->params.at("enc." + std::to_string(i) + "." + kAdapted[w]);
         const AdapterSet& ad = e->adapters[i * 4 + w];
         const size_t a = (size_t)e->adapter_rank * pi.cols, b = (size_t)e->adapter_rank * pi.rows;
-        ck(cudaMemset(ad.a + slot * a, 0, a * 2), "adapter clear");
-        ck(cudaMemset(ad.b + slot * b, 0, b * 2), "adapter clear");
-        ck(cudaMemset(ad.scaling + slot, 0, 4), "adapter clear");
+        ck(cudaMemsetAsync(ad.a + slot * a, 0, a * 2, e->stream), "adapter clear");
+        ck(cudaMemsetAsync(ad.b + slot * b, 0, b * 2, e->stream), "adapter clear");
+        ck(cudaMemsetAsync(ad.scaling + slot, 0, 4, e->stream), "adapter clear");
       }
-    ck(cudaDeviceSynchronize(), "adapter clear");
+    ck(cudaStreamSynchronize(e->stream), "adapter clear");
   });
 }
 
