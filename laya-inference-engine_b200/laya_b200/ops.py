@@ -123,7 +123,8 @@ def lora_linear_fp8(codes, scale, weight, weight_scale, x, lora_a, lora_b, index
 
 def op_status(device=None):
     """Nonzero when a bounded wait inside an operator ran out on ``device``
-    since the last call (its output is invalid); synchronises the device."""
+    since the last call (its output is invalid); synchronises the device, so not
+    while any thread captures a graph there."""
     with torch.cuda.device(device):
         torch.cuda.synchronize()
         status, lib = ctypes.c_int32(), _lib.load()
