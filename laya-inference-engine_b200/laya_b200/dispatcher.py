@@ -271,7 +271,9 @@ class B200Dispatcher:
                 # change that began without it has to be over, and none may begin.
                 with self._changes:
                     try:
-                        for name in {*self.adapters, *getattr(self.engines[d], "adapters", ())}:
+                        # (what was unloaded first: its slot may be needed)
+                        gone = set(getattr(self.engines[d], "adapters", ())) - set(self.adapters)
+                        for name in (*gone, *self.adapters):
                             self._restore(d, name)
                     except Exception:
                         continue

@@ -158,3 +158,26 @@ def test_load_without_a_healthy_gpu():
         assert e[0].adapters == e[1].adapters == {"a": 2.0}
         d.unload_adapter("a")
         assert e[0].adapters == e[1].adapters == {}
+
+
+@pytest.mark.parametrize("names", [("old", "new"), ("a", "b"), ("b", "a"), ("x", "y"), ("q1", "q0")])
+def test_restored_with_every_slot_in_use(names):
+    """What was unloaded meanwhile leaves its slot before the rest is loaded."""
+    old, new = names
+    d, e = dispatcher()
+    for engine in e.values():
+        loads = engine.load_adapter
+
+        def limited(name, *rest, engine=engine, loads=loads):
+            if name not in engine.adapters and len(engine.adapters) == 2:
+                raise RuntimeError("no adapter slot is free")
+            loads(name, *rest)
+
+        engine.load_adapter = limited
+    with d:
+        d.load_adapter("kept", PAIR)
+        d.load_adapter(old, PAIR)
+        drop_gpu_1(d, e)
+        d.unload_adapter(old)
+        d.load_adapter(new, PAIR)
+        assert d.readmit(items(None)) == [1] and e[1].adapters == e[0].adapters == {"kept": 1.0, new: 1.0}
